@@ -36,6 +36,20 @@ int nm_norm_bwd_device_status(void* stream, uint32_t* status_host);
  * afterwards nm_norm_bwd_device_status reports what a kernel whose wait ran out would have left. */
 int nm_norm_bwd_test_timeout(int64_t limit_cycles, void* stream);
 
+/* ---- embedding (the reference's trunk has its own, src/kernels/elementwise/embed.cu; names and workspace here are this
+ * library's). dtype: storage of table / out / dy, 1 = bf16, 0 = f32. D % 8 == 0, rows contiguous and 16-byte aligned.
+ * forward:  out[t, :] = round(scale * table[tokens[t], :]), one rounding; a token outside [0, V) gives a row of zeros. */
+int nm_embed_fwd(int dtype, const void* table, const int32_t* tokens, void* out, float scale, int64_t T, int D, int V,
+                 void* stream);
+/* backward: dtable[v, :] (f32 [V, D]) = or += scale * sum over t with tokens[t] = v of dy[t, :]. accumulate 0 writes all
+ * V rows (zeros for absent tokens), 1 adds and leaves absent rows untouched (a tied head's dW may be the buffer); tokens
+ * outside [0, V) contribute nothing. Sums are f32 in an order that depends on the tokens alone: the same call gives the
+ * same bits. workspace: nm_embed_bwd_workspace_bytes (0 on error), 256-byte aligned, scratch between calls; calls that may
+ * overlap need one each. Nothing is allocated; the calls can be captured into a CUDA graph. */
+uint64_t nm_embed_bwd_workspace_bytes(int64_t T, int D, int V);
+int nm_embed_bwd(int dtype, const void* dy, const int32_t* tokens, float* dtable, float scale, int accumulate, int64_t T,
+                 int D, int V, void* workspace, uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

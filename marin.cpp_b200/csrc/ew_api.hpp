@@ -56,6 +56,13 @@ void sandwich_tail_bwd_f32(const float* dx_out, const float* da_next, const floa
                            float* dx_in, float* dbranch, float* pg_next, float* pg_post, int64_t T, int D, float eps,
                            cudaStream_t st);
 
+// Embedding lookup with scaling and its gradient by sorted tokens (ew_embed.cu); what they promise: capi_ew.h.
+void embed_fwd(bool bf16, const void* table, const int32_t* tokens, void* out, float scale, int64_t T, int D, int V,
+               cudaStream_t st);
+uint64_t embed_bwd_workspace_bytes(int64_t T, int D, int V);
+void embed_bwd(bool bf16, const void* dy, const int32_t* tokens, float* dtable, float scale, bool accumulate, int64_t T,
+               int D, int V, void* ws, uint64_t ws_bytes, cudaStream_t st);
+
 // The word the norm backward kernels OR their error bits into when one of their bounded waits runs out (one per GPU,
 // zero-initialised, address looked up on first use: make the first backward call on a device outside a stream capture).
 // read_row_status copies it to the host after the stream's work, clears it when set, and returns it.
