@@ -52,6 +52,23 @@ struct Eight<false> {
   }
 };
 
+// Eight f32 values in one 32-byte store (sm_100): two 16-byte stores of a thread cover half of every 32-byte sector each.
+__device__ __forceinline__ void store32(float* p, const float* f) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]),
+               "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+               : "memory");
+}
+// p[0 .. 8) += f without reading p back: one addition per element and launch (every row has one writer), performed at L2,
+// so the result does not depend on any order. Additions at L2 flush values below 2^-126 to zero.
+__device__ __forceinline__ void add32(float* p, const float* f) {
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + 4), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]) : "memory");
+}
+// Between dependent launches of one call: the next kernel's CTAs may be set up while this one drains (`release`), and
+// wait for its completion before they touch what it wrote (`after_previous`).
+__device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------------------------------------------------------------------------ forward
 // G threads side by side on a row (eight elements each), kRows rows per group in flight: bound by HBM.
 constexpr int kFwdRows = 4;
@@ -83,16 +100,14 @@ __global__ void __launch_bounds__(kThreads) k_embed_fwd(const void* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------ sort
-// One cluster of up to eight CTAs sorts the positions of a section by token: a least-significant-digit radix sort, nine
+// One cluster of up to sixteen CTAs sorts the positions of a section by token: a least-significant-digit radix sort, nine
 // bits a pass, whose items never leave shared memory between passes (a pass scatters them into the other CTAs' shared
 // memory). CTA r holds the items [r * per, (r + 1) * per). Within a pass a warp ranks its items of equal digit by
-// match.any, 32 consecutive items at a time, which keeps the sort stable. The remaining CTAs of the grid have nothing to
-// sort; they zero the gradient rows of absent tokens when the call overwrites (the larger part of the writes when the
-// vocabulary is larger than the section), so the sort costs no time of its own there.
+// match.any, 32 consecutive items at a time, which keeps the sort stable.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kDigitBits = 9, kDigits = 1 << kDigitBits;
-constexpr int kMaxCluster = 8, kMaxPerThread = 16;
+constexpr int kMaxCluster = 16, kMaxPerThread = 8, kPosBits = 17;
 constexpr int64_t kSection = int64_t(kMaxCluster) * kSortThreads * kMaxPerThread;   // 131072 tokens
-constexpr int kZeroSlab = 65536;   // vocabulary rows whose presence a zeroing CTA marks at a time (8 KiB of bits)
+static_assert(kSection <= (int64_t(1) << kPosBits), "a position and its rank within a warp share one register");
 
 struct SortParams {
   const int32_t* tokens;
@@ -100,7 +115,6 @@ struct SortParams {
   int32_t* keys;        // [n] sorted tokens (V for one outside [0, V))
   int32_t* pos;         // [n] their positions
   int32_t* chains;      // word 0: how many long runs the reduction has listed (zeroed here)
-  float* dtable;        // rows to zero, or nullptr
   int cluster;          // CTAs that sort
 };
 
@@ -121,36 +135,90 @@ inline __host__ __device__ uint32_t sort_smem_bytes(int per) {
   return uint32_t(per) * 8u + kSortWarps * kDigits * 2u + 3u * kDigits * 4u + 128u;
 }
 
-__device__ void zero_absent_rows(const SortParams& p, uint32_t* bits) {
-  const int z = int(blockIdx.x) - p.cluster, zs = int(gridDim.x) - p.cluster;
-  const int v_begin = int(int64_t(p.V) * z / zs), v_end = int(int64_t(p.V) * (z + 1) / zs);
+// A short section (at most kRankMax tokens) needs no radix passes: the place of a token in the sorted order is the number
+// of tokens that are smaller, or equal and earlier. 32 positions per CTA, one per lane; warp w counts over the w-th eighth
+// of the tokens, which lie in shared memory.
+constexpr int kRankMax = 4096, kRankWarps = kThreads / 32;
+__global__ void __launch_bounds__(kThreads) k_embed_rank(const SortParams p) {
+  __shared__ __align__(16) int32_t key[kRankMax];
+  __shared__ int partial[kRankWarps][32];
+  release_next();
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.chains[0] = 0;
+  const int n4 = (p.n + 3) / 4;
+  for (int t = threadIdx.x; t < 4 * n4; t += kThreads) key[t] = t < p.n ? key_of(p, t) : INT_MAX;
+  __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int v0 = v_begin; v0 < v_end; v0 += kZeroSlab) {
-    const int rows = min(kZeroSlab, v_end - v0);
+  const int t = int(blockIdx.x) * 32 + lane;
+  const int k = t < p.n ? key[t] : 0;
+  int count = 0;
+#pragma unroll 4
+  for (int q = n4 * warp / kRankWarps; q < n4 * (warp + 1) / kRankWarps; ++q) {
+    const int4 v = reinterpret_cast<const int4*>(key)[q];
+    const int j = 4 * q;
+    count += (v.x < k || (v.x == k && j < t)) + (v.y < k || (v.y == k && j + 1 < t)) +
+             (v.z < k || (v.z == k && j + 2 < t)) + (v.w < k || (v.w == k && j + 3 < t));
+  }
+  partial[warp][lane] = count;
+  __syncthreads();
+  if (warp == 0 && t < p.n) {
+    int rank = 0;
+#pragma unroll
+    for (int w = 0; w < kRankWarps; ++w) rank += partial[w][lane];
+    p.keys[rank] = k;
+    p.pos[rank] = t;
+  }
+}
+
+// Zeroes the rows that no token of the section names (the larger part of the writes of an overwriting call whose
+// vocabulary is larger than the section). It needs the tokens, not their order, so it runs beside the sort: it does not wait
+// for the launch before it until it has done its work. The vocabulary is dealt to the CTAs (a power of two of them) in
+// blocks of eight rows, because frequent ids lie together; a CTA marks the tokens of its share, then writes.
+constexpr int kZeroThreads = 1024, kZeroSlab = 65536;   // rows whose presence a CTA marks at a time (8 KiB of bits)
+struct ZeroParams {
+  const int32_t* tokens;
+  float* dtable;
+  int n, V, D, log_ctas, wide;
+};
+__global__ void __launch_bounds__(kZeroThreads) k_embed_zero_absent(const ZeroParams p) {
+  __shared__ uint32_t bits[kZeroSlab / 32];
+  release_next();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t me = blockIdx.x, mask = gridDim.x - 1u;
+  // id v: block v >> 3 belongs to CTA (v >> 3) & mask, where it is row ((v >> 3) >> log_ctas) * 8 + (v & 7)
+  const int64_t slab_ids = int64_t(kZeroSlab) << p.log_ctas;
+  for (int64_t v0 = 0; v0 < p.V; v0 += slab_ids) {
+    const int ids = int(min(slab_ids, int64_t(p.V) - v0));
+    const int rows = (((ids + 7) >> 3) + int(mask) >> p.log_ctas) * 8;
     __syncthreads();
-    for (int i = threadIdx.x; i < (rows + 31) / 32; i += kSortThreads) bits[i] = 0u;
+    for (int i = threadIdx.x; i < (rows + 31) / 32; i += kZeroThreads) bits[i] = 0u;
     __syncthreads();
-#pragma unroll 8
-    for (int t = threadIdx.x; t < p.n; t += kSortThreads) {
-      const uint32_t at = uint32_t(__ldg(p.tokens + t) - v0);
-      if (at < uint32_t(rows)) atomicOr(&bits[at >> 5], 1u << (at & 31));
+#pragma unroll 16
+    for (int t = threadIdx.x; t < p.n; t += kZeroThreads) {
+      const int64_t v = int64_t(__ldg(p.tokens + t)) - v0;
+      if (v < 0 || v >= ids || ((uint32_t(v) >> 3) & mask) != me) continue;
+      const uint32_t at = (uint32_t(v) >> (3 + p.log_ctas)) * 8u + (uint32_t(v) & 7u), bit = 1u << (at & 31);
+      if (!(bits[at >> 5] & bit)) atomicOr(&bits[at >> 5], bit);   // a frequent token finds its bit set already
     }
     __syncthreads();
-    for (int r = warp; r < rows; r += kSortWarps) {
-      if ((bits[r >> 5] >> (r & 31)) & 1u) continue;
-      float4* row = reinterpret_cast<float4*>(p.dtable + int64_t(v0 + r) * p.D);
-      for (int c = lane; c < p.D / 4; c += 32) row[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = warp; r < rows; r += kZeroThreads / 32) {
+      const int64_t v = v0 + ((int64_t(r >> 3) << p.log_ctas) + me) * 8 + (r & 7);
+      if (v >= p.V || ((bits[r >> 5] >> (r & 31)) & 1u)) continue;
+      float* row = p.dtable + v * p.D;
+      const float none[8] = {};
+      if (p.wide) {
+        for (int c = lane * 8; c < p.D; c += 256) store32(row + c, none);
+      } else {
+        for (int c = lane * 8; c < p.D; c += 256) Eight<false>::store(row, c, none);
+      }
     }
   }
+  after_previous();
 }
 
 template <int R>   // items per thread
 __global__ void __launch_bounds__(kSortThreads, 1) k_embed_sort(const SortParams p) {
   extern __shared__ __align__(16) uint8_t sort_smem[];
-  if (int(blockIdx.x) >= p.cluster) {   // whole clusters: none of their CTAs sorts
-    zero_absent_rows(p, reinterpret_cast<uint32_t*>(sort_smem));
-    return;
-  }
+  release_next();
   using namespace nm::ptx;
   int32_t* buf = reinterpret_cast<int32_t*>(sort_smem);                        // [2][per] positions
   uint16_t* whist = reinterpret_cast<uint16_t*>(buf + 2 * p.per);              // [warps][digits]
@@ -168,24 +236,23 @@ __global__ void __launch_bounds__(kSortThreads, 1) k_embed_sort(const SortParams
     for (int i = threadIdx.x; i < kSortWarps * kDigits / 2; i += kSortThreads) wh[i] = 0u;
     __syncthreads();
     uint16_t* mine = whist + warp * kDigits;
-    int item[R], digit[R], rk[R];
+    int item[R], key[R];   // item: position, later with the rank among the warp's items of equal digit above it
+    uint32_t on = 0;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       const int at = warp * (32 * R) + j * 32 + lane;
-      const bool on = base + at < p.n;
-      item[j] = !on ? -1 : pass == 0 ? base + at : in[at];
+      if (base + at < p.n) on |= 1u << j;
+      item[j] = !((on >> j) & 1u) ? 0 : pass == 0 ? base + at : in[at];
     }
 #pragma unroll
-    for (int j = 0; j < R; ++j) digit[j] = item[j] >= 0 ? (key_of(p, item[j]) >> shift) & (kDigits - 1) : -1;
+    for (int j = 0; j < R; ++j) key[j] = ((on >> j) & 1u) ? key_of(p, item[j]) : -1;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const uint32_t same = __match_any_sync(0xffffffffu, digit[j]);
-      rk[j] = 0;
-      if (digit[j] >= 0) {
-        rk[j] = mine[digit[j]] + __popc(same & ((1u << lane) - 1u));
-      }
+      const int digit = ((on >> j) & 1u) ? (key[j] >> shift) & (kDigits - 1) : -1;
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      if (digit >= 0) item[j] |= (mine[digit] + __popc(same & ((1u << lane) - 1u))) << kPosBits;
       __syncwarp();
-      if (digit[j] >= 0 && lane == __ffs(same) - 1) mine[digit[j]] = uint16_t(mine[digit[j]] + __popc(same));
+      if (digit >= 0 && lane == __ffs(same) - 1) mine[digit] = uint16_t(mine[digit] + __popc(same));
       __syncwarp();
     }
     __syncthreads();
@@ -230,13 +297,14 @@ __global__ void __launch_bounds__(kSortThreads, 1) k_embed_sort(const SortParams
     const uint32_t out = smem_u32(buf + ((pass + 1) & 1) * p.per);
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      if (item[j] < 0) continue;
-      const int dest = start[digit[j]] + mine[digit[j]] + rk[j];
+      if (!((on >> j) & 1u)) continue;
+      const int digit = (key[j] >> shift) & (kDigits - 1), at = item[j] & ((1 << kPosBits) - 1);
+      const int dest = start[digit] + mine[digit] + (item[j] >> kPosBits);
       if (last) {
-        p.pos[dest] = item[j];
-        p.keys[dest] = key_of(p, item[j]);
+        p.pos[dest] = at;
+        p.keys[dest] = key[j];
       } else {
-        st_cluster(mapa_shared(out + 4u * uint32_t(dest & (p.per - 1)), uint32_t(dest >> log_per)), item[j]);
+        st_cluster(mapa_shared(out + 4u * uint32_t(dest & (p.per - 1)), uint32_t(dest >> log_per)), at);
       }
     }
     // the scattered items have landed; also: no CTA leaves while another may still read its counts
@@ -245,14 +313,16 @@ __global__ void __launch_bounds__(kSortThreads, 1) k_embed_sort(const SortParams
 }
 
 // ------------------------------------------------------------------------------------------------ reduction
-// The sorted positions are cut into windows of kWin; G threads (eight columns each) sum the rows of a window run by run.
-// A run that crosses a window's edge is finished by the window it began in, unless it extends at least kHalf to both
+// The sorted positions are cut into windows of `win`; G threads (eight columns each) sum the rows of a window run by run.
+// A run that crosses a window's edge is finished by the window it began in, unless it extends at least win / 2 to both
 // sides of the edge: then it is cut there, and each piece's sum goes to a row of its own in the workspace (slot 0 of a
 // window: a piece that continues a run; slot 1: a piece that begins one), to be joined afterwards in order. So short
-// runs are never cut, no window has more than 2.5 kWin rows to read, and a cut costs 8 bytes of f32 traffic per column
-// for at least kWin / 2 rows read.
-constexpr int kWin = 32, kHalf = kWin / 2, kSpan = 3 * kWin;
+// runs are never cut, no window has more than 2.5 win rows to read, and a cut costs 8 bytes of f32 traffic per column
+// for at least win / 2 rows read.
 constexpr int kNoKey = INT_MAX;
+// Measured for 131072 tokens of width 2048 (ids falling as 1 / rank): windows of 64 rows 297 us for the whole call, of 32
+// rows 305 us (twice the cut pieces). Short sections take 32: there are then enough windows to fill the SMs.
+inline int window_for(int64_t n) { return n > 32768 ? 64 : 32; }
 
 struct ReduceParams {
   const void* dy;
@@ -261,156 +331,256 @@ struct ReduceParams {
   float* part;          // [windows][2][D]
   float* dtable;
   float scale;
-  int n, V, D, G, windows, accumulate;
+  int n, V, D, G, win, windows, accumulate, wide;   // wide: rows of dtable and part are 32-byte aligned
 };
 
 // Is the run that holds sorted index b cut at b? `key(i)` reads the sorted keys (kNoKey outside).
 template <class Key>
-__device__ __forceinline__ bool is_cut(const Key& key, int b, int V) {
+__device__ __forceinline__ bool is_cut(const Key& key, int b, int win, int V) {
   const int k = key(b);
-  return b > 0 && k < V && key(b - 1) == k && key(b - kHalf) == k && key(b + kHalf - 1) == k;
+  return b > 0 && k < V && key(b - 1) == k && key(b - win / 2) == k && key(b + win / 2 - 1) == k;
 }
 // First index the window at b owns: b itself at the start of a run or at a cut, else the end of the run that b lies in
 // (the window before finishes it) or the next edge when the run is cut there. Whole warps call it.
 template <class Key>
-__device__ __forceinline__ int first_owned(const Key& key, int b, int V, int lane) {
+__device__ __forceinline__ int first_owned(const Key& key, int b, int win, int V, int lane) {
   const int k = key(b);
-  if (b == 0 || k >= V || key(b - 1) != k || is_cut(key, b, V)) return b;
-  for (int o = 0; o < kWin + kHalf; o += 32) {
+  if (b == 0 || k >= V || key(b - 1) != k || is_cut(key, b, win, V)) return b;
+  for (int o = 0; o < win + win / 2; o += 32) {
     const uint32_t other = __ballot_sync(0xffffffffu, key(b + o + lane) != k);
     if (other) {
       const int e = b + o + __ffs(other) - 1;
-      return (e > b + kWin && is_cut(key, b + kWin, V)) ? b + kWin : e;
+      return (e > b + win && is_cut(key, b + win, win, V)) ? b + win : e;
     }
   }
-  return b + kWin;   // the run extends further: it is cut at the next edge
+  return b + win;   // the run extends further: it is cut at the next edge
 }
 
-template <bool BF16, int U>
-__global__ void __launch_bounds__(kThreads) k_embed_reduce(const ReduceParams p) {
-  __shared__ int32_t skey[(kThreads / 32) * kSpan];
-  __shared__ int32_t spos[(kThreads / 32) * kSpan];
+// A thread's pieces of the rows to come travel through its own slots of a ring in shared memory (cp.async, no barrier:
+// nobody else reads them), 64 KiB in flight per CTA: what a window waits for is a few round trips, and registers do not
+// limit how many rows are on their way.
+template <bool BF16>
+struct Ring {
+  static constexpr int kGroups = 4;                        // commit groups in flight
+  static constexpr int kRows = BF16 ? 4 : 2;               // rows per group
+  static constexpr int kPieces = BF16 ? 1 : 2;             // 16-byte pieces per row and thread
+  static constexpr int kBytes = kGroups * kRows * kPieces * kThreads * 16;
+};
+// 16 bytes, or zeros without a read when `bytes` is 0
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Shared memory of the reduction: the ring, then per row group the keys and the rows of its window (in 16-byte units from
+// dy), padded to whole ring groups.
+inline __host__ __device__ int span_of(int win) { return 3 * win; }
+template <bool BF16>
+int reduce_smem_bytes(int groups, int win) { return Ring<BF16>::kBytes + groups * span_of(win) * 3 * 4; }
+
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads, 3) k_embed_reduce(const ReduceParams p) {
+  using R = Ring<BF16>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ int ends[kThreads / 32];
+  release_next();
   const int groups = kThreads / p.G, g = threadIdx.x / p.G, tg = threadIdx.x % p.G, lane = threadIdx.x & 31;
-  const int win = int(blockIdx.x) * groups + g;
-  const int b = win * kWin, origin = b - kHalf;
-  int32_t* const k_s = skey + g * kSpan;
-  int32_t* const p_s = spos + g * kSpan;
-  for (int i = tg; i < kSpan; i += p.G) {
+  const int win = int(blockIdx.x) * groups + g, W = p.win, span = span_of(W);
+  const int b = win * W, origin = b - W / 2;
+  int32_t* const k_s = reinterpret_cast<int32_t*>(ring + R::kBytes) + g * span * 3;   // keys of the span
+  int32_t* const m_s = k_s + span;      // per row: the key where a piece ends, -1 elsewhere
+  uint32_t* const r_s = reinterpret_cast<uint32_t*>(m_s + span);
+  after_previous();
+  for (int i = tg; i < span; i += p.G) {
     const int at = origin + i;
-    const bool on = at >= 0 && at < p.n;
-    k_s[i] = on ? __ldg(p.keys + at) : kNoKey;
-    p_s[i] = on ? __ldg(p.pos + at) : 0;
+    k_s[i] = at >= 0 && at < p.n ? __ldcg(p.keys + at) : kNoKey;
   }
   __syncthreads();
-  if (win >= p.windows) return;
   // an index at or beyond the span is never reached by a run that is not cut before; it reads as "another key"
   auto key = [&](int i) {
     const int at = i - origin;
-    return at >= 0 && at < kSpan ? k_s[at] : kNoKey;
+    return at >= 0 && at < span ? k_s[at] : kNoKey;
   };
-  const int begin = first_owned(key, b, p.V, lane);
-  const int end = min(p.n, first_owned(key, b + kWin, p.V, lane));
-  if (begin >= end || key(begin) >= p.V) return;
-  const int pc = blockIdx.y * p.G + tg;
-  const bool on = pc * 8 < p.D;
-  bool continues = is_cut(key, b, p.V) && begin == b;       // the first piece continues a run of the window before
-  const bool cut_end = is_cut(key, end, p.V);               // the last piece goes on in the next window
+  int begin = 0, end = 0;
+  if (win < p.windows) {
+    begin = first_owned(key, b, W, p.V, lane);
+    end = min(p.n, first_owned(key, b + W, W, p.V, lane));
+  }
+  const bool work = begin < end && key(begin) < p.V;
+  const bool continues = work && begin == b && is_cut(key, b, W, p.V);   // the first piece continues a run
+  const bool cut_end = work && is_cut(key, end, W, p.V);                 // the last piece goes on in the next window
   if (cut_end && tg == 0 && blockIdx.y == 0 && !(continues && key(begin) == key(end - 1)))
     p.chains[1 + atomicAdd(p.chains, 1)] = win;
-  float acc[8] = {};
-  for (int i0 = begin; i0 < end; i0 += U) {
-    Eight<BF16> e[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (on && i0 + u < end && key(i0 + u) < p.V) e[u].load(p.dy, int64_t(p_s[i0 + u - origin]) * p.D + pc * 8);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u;
-      if (i >= end) break;
-      const int k = key(i);
-      if (k >= p.V) return;                                  // ids outside the vocabulary sort last
-      float f[8];
-      if (on) e[u].get(f);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) acc[q] += f[q];
-      const bool piece_end = i + 1 >= end || key(i + 1) != k;
-      if (piece_end) {
-        if (on) {
-          const bool goes_on = i + 1 >= end && cut_end;
-          if (continues || goes_on) {
-            Eight<false>::store(p.part, (int64_t(win) * 2 + (continues ? 0 : 1)) * p.D + pc * 8, acc);
-          } else {
-            const int64_t at = int64_t(k) * p.D + pc * 8;
-            float o[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q) o[q] = p.scale * acc[q];
-            if (p.accumulate) {
-              Eight<false> old;
-              const float4* s = reinterpret_cast<const float4*>(p.dtable + at);
-              old.a = s[0], old.b = s[1];
-              float w[8];
-              old.get(w);
-#pragma unroll
-              for (int q = 0; q < 8; ++q) o[q] += w[q];
-            }
-            Eight<false>::store(p.dtable, at, o);
-          }
-        }
-        continues = false;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] = 0.f;
-      }
+  const int first_key = work ? key(begin) : kNoKey, last_key = work ? key(end - 1) : kNoKey;
+  if (tg == 0) ends[g] = end;
+  __syncthreads();
+  if (work) {
+    for (int i = begin + tg; i < begin + span; i += p.G) {
+      const int k = i < end ? key(i) : kNoKey;
+      if (i < end && k >= p.V && key(i - 1) < p.V) ends[g] = i;   // ids outside the vocabulary sort last
+      const int next = i + 1 < end ? key(i + 1) : kNoKey;
+      m_s[i - begin] = k < p.V && next != k ? k : -1;
+      r_s[i - begin] = k < p.V ? uint32_t(__ldcg(p.pos + i)) * uint32_t(p.D / 8 * R::kPieces) : 0u;
     }
   }
+  __syncthreads();
+  const int col = (blockIdx.y * p.G + tg) * 8;
+  if (!work || col >= p.D) return;
+  const int rows = ends[g] - begin;
+  const uint32_t slots = nm::ptx::smem_u32(ring) + threadIdx.x * 16u;
+  auto slot = [&](int group, int u, int piece) {
+    return slots + uint32_t(((group * R::kRows + u) * R::kPieces + piece) * kThreads) * 16u;
+  };
+  const uint8_t* const mine = static_cast<const uint8_t*>(p.dy) + int64_t(col) * (BF16 ? 2 : 4);
+  auto fetch = [&](int group, int i0) {       // rows past the end become zeros
+#pragma unroll
+    for (int u = 0; u < R::kRows; ++u) {
+      const bool in = i0 + u < rows;
+      const uint8_t* src = mine + (in ? uint64_t(r_s[i0 + u]) * 16u : 0u);
+#pragma unroll
+      for (int h = 0; h < R::kPieces; ++h) cp_async16(slot(group, u, h), src + 16 * h, in ? 16u : 0u);
+    }
+    cp_async_commit();
+  };
+  F2 acc[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) acc[q] = f2(0.f, 0.f);
+  auto flush = [&](int k) {
+    float* to;
+    float f[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f2_get(acc[q], f[2 * q], f[2 * q + 1]), acc[q] = f2(0.f, 0.f);
+    const bool head = continues && k == first_key, tail = cut_end && k == last_key;
+    if (head || tail) {
+      to = p.part + (int64_t(win) * 2 + (head ? 0 : 1)) * p.D + col;
+    } else {
+      to = p.dtable + int64_t(k) * p.D + col;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) f[q] *= p.scale;
+    }
+    if (p.accumulate && !head && !tail) {
+      add32(to, f);
+    } else if (p.wide) {
+      store32(to, f);
+    } else {
+      Eight<false>::store(to, 0, f);
+    }
+  };
+#pragma unroll
+  for (int g4 = 0; g4 < R::kGroups; ++g4) fetch(g4, g4 * R::kRows);
+  for (int i0 = 0; i0 < rows;) {
+#pragma unroll
+    for (int group = 0; group < R::kGroups; ++group) {
+      cp_async_wait<R::kGroups - 1>();
+#pragma unroll
+      for (int u = 0; u < R::kRows; ++u) {
+        const int m = i0 + u < rows ? m_s[i0 + u] : -1;
+        const uint4 q0 = nm::ptx::ld_shared_v4(slot(group, u, 0));
+        if constexpr (BF16) {
+          acc[0] = f2_add(acc[0], f2_of(q0.x)), acc[1] = f2_add(acc[1], f2_of(q0.y));
+          acc[2] = f2_add(acc[2], f2_of(q0.z)), acc[3] = f2_add(acc[3], f2_of(q0.w));
+        } else {
+          const uint4 q1 = nm::ptx::ld_shared_v4(slot(group, u, 1));
+          acc[0] = f2_add(acc[0], f2(__uint_as_float(q0.x), __uint_as_float(q0.y)));
+          acc[1] = f2_add(acc[1], f2(__uint_as_float(q0.z), __uint_as_float(q0.w)));
+          acc[2] = f2_add(acc[2], f2(__uint_as_float(q1.x), __uint_as_float(q1.y)));
+          acc[3] = f2_add(acc[3], f2(__uint_as_float(q1.z), __uint_as_float(q1.w)));
+        }
+        if (m >= 0) flush(m);
+      }
+      fetch(group, i0 + R::kGroups * R::kRows);
+      i0 += R::kRows;
+    }
+  }
+  cp_async_wait<0>();
 }
 
-// Joins the pieces of the listed cut runs: slot 1 of the window the run begins in, then slot 0 of the windows after it,
-// in that order dealt to eight row lanes whose sums are added in lane order. 32 threads side by side on 128 columns.
-constexpr int kJoinCols = 128, kJoinLanes = kThreads / 32;
+// Joins the pieces of the listed cut runs: slot 1 of the window the run begins in, then slot 0 of the windows after it, in
+// that order. A job is 128 columns of one run and belongs to a warp; a run of more than kJoinAlone pieces is summed by all
+// warps of the CTA together (pieces dealt to the warps, their sums added in warp order), so that what the launch takes is
+// a few round trips whatever the longest run.
+constexpr int kJoinCols = 128, kJoinWarps = kThreads / 32, kJoinAlone = 16;
+struct JoinJob {
+  int win, second, pieces, col, key;
+};
+__device__ __forceinline__ float4 add4(float4 a, float4 b) {
+  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+__device__ __forceinline__ float4 join_pieces(const ReduceParams& p, const JoinJob& j, int col, int from, int step) {
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < p.D) {
+#pragma unroll 8
+    for (int i = from; i < j.pieces; i += step) {
+      const int64_t slot = i == 0 ? int64_t(j.win) * 2 + 1 : int64_t(j.second + i - 1) * 2;
+      s = add4(s, __ldcg(reinterpret_cast<const float4*>(p.part + slot * p.D + col)));
+    }
+  }
+  return s;
+}
+__device__ __forceinline__ void join_write(const ReduceParams& p, int key, int col, float4 s) {
+  if (col >= p.D) return;
+  float4* o = reinterpret_cast<float4*>(p.dtable + int64_t(key) * p.D + col);
+  const float4 r = make_float4(p.scale * s.x, p.scale * s.y, p.scale * s.z, p.scale * s.w);
+  *o = p.accumulate ? add4(*o, r) : r;
+}
 __global__ void __launch_bounds__(kThreads) k_embed_join(const ReduceParams p) {
-  __shared__ float4 red[kJoinLanes][32];
-  const int count = p.chains[0];
+  __shared__ float4 red[kJoinWarps][32];
+  __shared__ JoinJob long_jobs[kJoinWarps];
+  __shared__ int n_long;
+  after_previous();
+  const int count = __ldcg(p.chains), half = p.win / 2;
   const int col_blocks = (p.D + kJoinCols - 1) / kJoinCols;
-  const int tc = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  for (int64_t job = blockIdx.x; job < int64_t(count) * col_blocks; job += gridDim.x) {
-    const int win = p.chains[1 + int(job / col_blocks)];
-    const int col = int(job % col_blocks) * kJoinCols + tc * 4;
-    const int edge = (win + 1) * kWin;
-    const int k = __ldg(p.keys + edge);
-    int lo = edge, hi = p.n;                       // end of the run: first index whose key is larger
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(p.keys + mid) > k) hi = mid;
-      else lo = mid + 1;
-    }
-    // the first cut: at this edge, or at the next one when the run has fewer than kHalf rows before this edge
-    const bool here = edge >= kHalf && __ldg(p.keys + edge - kHalf) == k && lo >= edge + kHalf;
-    const int second = here ? win + 1 : win + 2;   // the window that holds the second piece
-    const int last = (lo - kHalf) / kWin;          // the last edge inside the run with kHalf rows of it behind the edge
-    const int pieces = last - second + 2;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col < p.D) {
-#pragma unroll 4
-      for (int i = rl; i < pieces; i += kJoinLanes) {
-        const int64_t slot = i == 0 ? int64_t(win) * 2 + 1 : int64_t(second + i - 1) * 2;
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + slot * p.D + col));
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-      }
-    }
-    red[rl][tc] = s;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t jobs = int64_t(count) * col_blocks;
+  // jobs are dealt to the CTAs first: the column blocks of one long run go to different CTAs
+  for (int64_t job0 = blockIdx.x; job0 < jobs; job0 += int64_t(gridDim.x) * kJoinWarps) {
+    if (threadIdx.x == 0) n_long = 0;
     __syncthreads();
-    if (rl == 0 && col < p.D) {
-      for (int w = 1; w < kJoinLanes; ++w) {
-        const float4 v = red[w][tc];
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    const int64_t job = job0 + int64_t(warp) * gridDim.x;
+    if (job < jobs) {
+      JoinJob j;
+      j.win = __ldcg(p.chains + 1 + int(job / col_blocks));
+      j.col = int(job % col_blocks) * kJoinCols;
+      const int edge = (j.win + 1) * p.win;
+      const int k = __ldcg(p.keys + edge);
+      j.key = k;
+      // the first cut: at this edge, or at the next one when the run has fewer than half a window on a side of this edge
+      const bool here = edge >= half && __ldcg(p.keys + edge - half) == k && edge + half - 1 < p.n &&
+                        __ldcg(p.keys + edge + half - 1) == k;
+      j.second = here ? j.win + 1 : j.win + 2;   // the window that holds the second piece
+      // the edges after it at which the run is cut too: those with half a window of it behind them
+      j.pieces = 2;
+      for (int w0 = j.second + 1;; w0 += 128) {
+        int found = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t at = int64_t(w0 + q * 32 + lane) * p.win + half - 1;
+          found += __popc(__ballot_sync(0xffffffffu, at < p.n && __ldcg(p.keys + at) == k));
+        }
+        j.pieces += found;
+        if (found < 128) break;
       }
-      float4* o = reinterpret_cast<float4*>(p.dtable + int64_t(k) * p.D + col);
-      float4 r = make_float4(p.scale * s.x, p.scale * s.y, p.scale * s.z, p.scale * s.w);
-      if (p.accumulate) {
-        const float4 old = *o;
-        r.x += old.x, r.y += old.y, r.z += old.z, r.w += old.w;
+      const int col = j.col + lane * 4;
+      if (j.pieces <= kJoinAlone) join_write(p, k, col, join_pieces(p, j, col, 0, 1));
+      else if (lane == 0) long_jobs[atomicAdd(&n_long, 1)] = j;
+    }
+    __syncthreads();
+    const int longs = n_long;
+    for (int i = 0; i < longs; ++i) {            // in whatever order they were listed: they write different columns
+      const JoinJob j = long_jobs[i];
+      const int col = j.col + lane * 4;
+      red[warp][lane] = join_pieces(p, j, col, warp, kJoinWarps);
+      __syncthreads();
+      if (warp == 0) {
+        float4 s = red[0][lane];
+        for (int w = 1; w < kJoinWarps; ++w) s = add4(s, red[w][lane]);
+        join_write(p, j.key, col, s);
       }
-      *o = r;
+      __syncthreads();
     }
     __syncthreads();
   }
@@ -432,7 +602,7 @@ struct BwdRegions {
   uint64_t bytes;
 };
 BwdRegions bwd_layout(int64_t T, int D, void* base) {
-  const int64_t n = std::min(T, kSection), windows = (n + kWin - 1) / kWin;
+  const int64_t n = std::min(T, kSection), windows = (n + window_for(n) - 1) / window_for(n);
   ce::Arena arena(base);
   BwdRegions r{};
   r.keys = arena.take<int32_t>(uint64_t(n));
@@ -453,18 +623,36 @@ void require_arch(const char* who) {
   NM_REQUIRE(ce::device_arch() >= 100, std::string(who) + ": this library holds sm_100a code only");
 }
 
-template <int R>
-void launch_sort(const SortParams& p, int cluster, int grid, cudaStream_t st) {
-  const uint32_t smem = std::max(sort_smem_bytes(p.per), uint32_t(kZeroSlab / 8));
-  NM_CUDA(cudaFuncSetAttribute(k_embed_sort<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+// Launch whose CTAs may be set up while the launch before it drains; the kernel waits itself (after_previous).
+template <class Kernel, class Params>
+void launch_next(Kernel kernel, dim3 grid, int threads, int smem, const Params& p, cudaStream_t st) {
+  if (smem > 48 * 1024) NM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(grid));
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NM_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+template <int R>
+void launch_sort(const SortParams& p, cudaStream_t st) {
+  const uint32_t smem = sort_smem_bytes(p.per);
+  NM_CUDA(cudaFuncSetAttribute(k_embed_sort<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  NM_CUDA(cudaFuncSetAttribute(k_embed_sort<R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(p.cluster));
   cfg.blockDim = dim3(kSortThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = unsigned(cluster); attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  attr.val.clusterDim.x = unsigned(p.cluster); attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   NM_CUDA(cudaLaunchKernelEx(&cfg, k_embed_sort<R>, p));
@@ -525,29 +713,37 @@ void embed_bwd(bool bf16, const void* dy, const int32_t* tokens, float* dtable, 
     while (int64_t(per) * kMaxCluster < n) per *= 2;
     int cluster = 1;
     while (cluster * per < n) cluster *= 2;
-    SortParams sp{tokens + t0, n, V, D, per, (bits + kDigitBits - 1) / kDigitBits, r.keys, r.pos, r.chains,
-                  add ? nullptr : dtable, cluster};
-    const int grid = add ? cluster : cluster * std::max(2, ce::sm_count() / cluster);
-    switch (per / kSortThreads) {
-      case 1: launch_sort<1>(sp, cluster, grid, st); break;
-      case 2: launch_sort<2>(sp, cluster, grid, st); break;
-      case 4: launch_sort<4>(sp, cluster, grid, st); break;
-      case 8: launch_sort<8>(sp, cluster, grid, st); break;
-      default: launch_sort<16>(sp, cluster, grid, st); break;
+    SortParams sp{tokens + t0, n, V, D, per, (bits + kDigitBits - 1) / kDigitBits, r.keys, r.pos, r.chains, cluster};
+    if (n <= kRankMax) {
+      k_embed_rank<<<unsigned((n + 31) / 32), kThreads, 0, st>>>(sp);
+      NM_CUDA(cudaGetLastError());
+    } else {
+      switch (per / kSortThreads) {
+        case 1: launch_sort<1>(sp, st); break;
+        case 2: launch_sort<2>(sp, st); break;
+        case 4: launch_sort<4>(sp, st); break;
+        default: launch_sort<8>(sp, st); break;
+      }
+    }
+    const bool wide = reinterpret_cast<uintptr_t>(dtable) % 32 == 0;
+    if (!add) {   // at most one CTA on each SM that does not sort
+      int log_ctas = 0;
+      while ((2 << log_ctas) <= ce::sm_count() - (n > kRankMax ? cluster : 0)) ++log_ctas;
+      const ZeroParams zp{tokens + t0, dtable, n, V, D, log_ctas, wide};
+      launch_next(k_embed_zero_absent, dim3(1u << log_ctas), kZeroThreads, 0, zp, st);
     }
     ReduceParams rp{};
     rp.dy = static_cast<const uint8_t*>(dy) + t0 * D * (bf16 ? 2 : 4);
     rp.keys = r.keys, rp.pos = r.pos, rp.chains = r.chains, rp.part = r.part, rp.dtable = dtable, rp.scale = scale;
-    rp.n = n, rp.V = V, rp.D = D, rp.G = threads_per_row(D / 8), rp.windows = (n + kWin - 1) / kWin;
-    rp.accumulate = add;
+    rp.n = n, rp.V = V, rp.D = D, rp.G = threads_per_row(D / 8), rp.accumulate = add;
+    rp.win = window_for(n), rp.windows = (n + rp.win - 1) / rp.win;
+    rp.wide = wide;
     const int groups = kThreads / rp.G;
     const dim3 rg(unsigned((rp.windows + groups - 1) / groups), unsigned((D / 8 + rp.G - 1) / rp.G));
-    if (bf16) k_embed_reduce<true, 8><<<rg, kThreads, 0, st>>>(rp);
-    else k_embed_reduce<false, 4><<<rg, kThreads, 0, st>>>(rp);
-    NM_CUDA(cudaGetLastError());
+    if (bf16) launch_next(k_embed_reduce<true>, rg, kThreads, reduce_smem_bytes<true>(groups, rp.win), rp, st);
+    else launch_next(k_embed_reduce<false>, rg, kThreads, reduce_smem_bytes<false>(groups, rp.win), rp, st);
     const int64_t jobs = int64_t(rp.windows) * ((D + kJoinCols - 1) / kJoinCols);
-    k_embed_join<<<unsigned(std::min<int64_t>(jobs, int64_t(ce::sm_count()) * 4)), kThreads, 0, st>>>(rp);
-    NM_CUDA(cudaGetLastError());
+    launch_next(k_embed_join, dim3(unsigned(std::min<int64_t>(jobs, int64_t(ce::sm_count()) * 8))), kThreads, 0, rp, st);
   }
 }
 
