@@ -50,6 +50,32 @@ uint64_t nm_embed_bwd_workspace_bytes(int64_t T, int D, int V);
 int nm_embed_bwd(int dtype, const void* dy, const int32_t* tokens, float* dtable, float scale, int accumulate, int64_t T,
                  int D, int V, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---- gated sandwich tail: the norms before and after a block, fused with the block's gate and the scaled residual (the
+ * ungated tail is nm_sandwich_tail_fwd / _bwd, capi.h). dtype: storage of the row tensors, the gate and the gains, 1 = bf16
+ * (D <= 8192), 0 = f32 (D <= 4096); D % 8 == 0, rows contiguous, pointers 16-byte aligned (a gate per token: its element
+ * size). f32 inside, one rounding per stored output.
+ *   y = g_post ? g_post * branch * rstd_post : branch        rstd_post = 1 / sqrt(mean(branch^2) + eps)
+ *   x_out = round(res_scale * x_in + sigmoid(gate) * y)      gate_kind 0: no gate (NULL), 1: gate [T], 2: gate [T, D]
+ *   a_next = round(g_next * x_out * rstd_next)               rstd_next = 1 / sqrt(mean(x_out^2) + eps), of the rounded x_out
+ * NULL: res_scale ([D]; 1), g_post ([D]; no post-norm), a_next (then g_next too), rstd_post / rstd_next (not returned).
+ * x_out may be x_in and a_next may be branch. */
+int nm_gated_tail_fwd(int dtype, int gate_kind, const void* branch, const void* x_in, const void* gate,
+                      const void* res_scale, const void* g_post, const void* g_next, void* x_out, void* a_next,
+                      float* rstd_post, float* rstd_next, int64_t T, int D, float eps, void* stream);
+/* Gradients of dx_out (gradient that reaches x_out from elsewhere; NULL: none) and da_next with respect to x_in, branch,
+ * gate (dgate, same shape), and, each f32 [D] and overwritten, NULL to skip: g_next, g_post, res_scale. x_in, branch, gate,
+ * the gains and the statistics are those of the forward call (x_out is formed again and not needed). dx_in may be dx_out,
+ * dbranch may be branch, dgate may be gate. Sums have a fixed order: the same call gives the same bits. workspace
+ * (nm_gated_tail_workspace_bytes, 0 on error; not needed when no [D] gradient is asked for): scratch between calls; calls
+ * that may overlap need one each. Nothing is allocated. Waits of these two kernels are bounded: nm_norm_bwd_device_status
+ * reports one that ran out; make the first call on a device outside a stream capture. */
+uint64_t nm_gated_tail_workspace_bytes(int64_t T, int D);
+int nm_gated_tail_bwd(int dtype, int gate_kind, const void* dx_out, const void* da_next, const void* x_in,
+                      const void* branch, const void* gate, const void* res_scale, const void* g_post, const void* g_next,
+                      const float* rstd_post, const float* rstd_next, void* dx_in, void* dbranch, void* dgate,
+                      float* dg_next, float* dg_post, float* dres_scale, int64_t T, int D, void* workspace,
+                      uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -63,6 +63,16 @@ uint64_t embed_bwd_workspace_bytes(int64_t T, int D, int V);
 void embed_bwd(bool bf16, const void* dy, const int32_t* tokens, float* dtable, float scale, bool accumulate, int64_t T,
                int D, int V, void* ws, uint64_t ws_bytes, cudaStream_t st);
 
+// The gated sandwich tail (ew_gated.cu); what it computes and promises: capi_ew.h.
+void gated_tail_fwd(bool bf16, int gate_kind, const void* branch, const void* x_in, const void* gate, const void* res_scale,
+                    const void* g_post, const void* g_next, void* x_out, void* a_next, float* rstd_post, float* rstd_next,
+                    int64_t T, int D, float eps, cudaStream_t st);
+uint64_t gated_tail_workspace_bytes(int64_t T, int D);
+void gated_tail_bwd(bool bf16, int gate_kind, const void* dx_out, const void* da_next, const void* x_in, const void* branch,
+                    const void* gate, const void* res_scale, const void* g_post, const void* g_next, const float* rstd_post,
+                    const float* rstd_next, void* dx_in, void* dbranch, void* dgate, float* dg_next, float* dg_post,
+                    float* dres_scale, int64_t T, int D, void* ws, uint64_t ws_bytes, cudaStream_t st);
+
 // The word the norm backward kernels OR their error bits into when one of their bounded waits runs out (one per GPU,
 // zero-initialised, address looked up on first use: make the first backward call on a device outside a stream capture).
 // read_row_status copies it to the host after the stream's work, clears it when set, and returns it.

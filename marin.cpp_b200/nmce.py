@@ -61,6 +61,10 @@ SIGS = {
     "nm_embed_fwd": (I32, [I32, VP, VP, VP, F32, I64, I32, I32, VP]),
     "nm_embed_bwd_workspace_bytes": (U64, [I64, I32, I32]),
     "nm_embed_bwd": (I32, [I32, VP, VP, VP, F32, I32, I64, I32, I32, VP, U64, VP]),
+    "nm_gated_tail_fwd": (I32, [I32, I32, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, I64, I32, F32, VP]),
+    "nm_gated_tail_workspace_bytes": (U64, [I64, I32]),
+    "nm_gated_tail_bwd": (I32, [I32, I32, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, I64, I32, VP, U64,
+                                VP]),
     "nm_comm_unique_id": (I32, [VP]),
     "nm_comm_create": (I32, [VP, I32, I32, VP]),
     "nm_comm_destroy": (I32, [VP]),
@@ -90,7 +94,7 @@ SIGS = {
 }
 NO_STATUS = {"nm_version", "nm_last_error", "nm_device_arch", "nm_ce_workspace_bytes", "nm_ce_set_backends",
              "nm_ce_device_arch", "nm_ce_set_fast_stats_exp", "nm_ce_sampled_stride", "nm_ce_sampled_workspace_bytes", "nm_norm_partial_rows", "nm_head_adamh_owned_elems", "nm_grad_reducer_owned_elems", "nm_ce_suggest_chunk_rows",
-             "nm_embed_bwd_workspace_bytes"}
+             "nm_embed_bwd_workspace_bytes", "nm_gated_tail_workspace_bytes"}
 
 IMPLS = {"A": 0, "B1": 1, "B1.5": 2, "B2": 3}
 LEV, ACC = 0, 1
