@@ -9,7 +9,7 @@
 // policy of the sandwich tail); x_out is what the residual stream holds, so the next norm reads its rounded values. The
 // backward forms x_out again from x_in, branch and gate instead of reading it: bit for bit the stored one, because both
 // directions share outer() below, and 2 bytes per element less.
-// sigmoid(g) and its derivative come from e = exp(-|g|), r = 1 / (1 + e): r or e r, and e r^2: no cancellation.
+// sigmoid(g) = r = 1 / (1 + e) and 1 - sigmoid(g) = e r with e = exp(-g): no cancellation at either end.
 // Row groups and batch ring as in ew_rows.cuh. What bounds them is HBM (10 and 16 bytes per element in bf16 with a gate per
 // element).
 #include <cuda_bf16.h>
@@ -29,84 +29,102 @@ namespace {
 
 enum GateKind : int { kNoGate = 0, kTokenGate = 1, kElementGate = 2 };
 
-// Eight consecutive elements: as stored, and as four f32 pairs.
+// A thread's unit is four columns: their operands are read from the slot and used at once (with eight, the operands alone
+// push the backward past its 128 registers). Warp w of a row group owns the quads [32 N w, 32 N (w + 1)), lane l of it the
+// quads l, l + 32, ...: neighbours side by side, and distances between a thread's quads that are constants.
 template <bool BF16>
-struct Raw {
-  static constexpr int kBytes = BF16 ? 16 : 32;
-  uint4 q[BF16 ? 1 : 2];
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (auto& v : q) v = make_uint4(0u, 0u, 0u, 0u);
+struct Quad {
+  uint32_t w[BF16 ? 2 : 4];
+  static constexpr uint32_t kBytes = BF16 ? 8 : 16;
+  __device__ __forceinline__ void fill(float v) {
+    const uint32_t u = __float_as_uint(v);
+    if constexpr (BF16) w[0] = w[1] = (u >> 16) | (u & 0xffff0000u);
+    else w[0] = w[1] = w[2] = w[3] = u;
   }
   __device__ __forceinline__ void from_shared(uint32_t at) {
-    q[0] = nm::ptx::ld_shared_v4(at);
-    if constexpr (!BF16) q[1] = nm::ptx::ld_shared_v4(at + 16u);
-  }
-  __device__ __forceinline__ void from_global(const void* p, int64_t element) {
-    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + element * (BF16 ? 2 : 4));
-    q[0] = __ldg(s);
-    if constexpr (!BF16) q[1] = __ldg(s + 1);
-  }
-  __device__ __forceinline__ void to_global(void* p, int64_t element) const {
-    uint4* d = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + element * (BF16 ? 2 : 4));
-    d[0] = q[0];
-    if constexpr (!BF16) d[1] = q[1];
-  }
-  __device__ __forceinline__ F2 pair(int i) const {
     if constexpr (BF16) {
-      return f2_of(word_of(q[0], i));
+      asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
     } else {
-      const uint4& h = q[i >> 1];
-      return (i & 1) ? f2(__uint_as_float(h.z), __uint_as_float(h.w)) : f2(__uint_as_float(h.x), __uint_as_float(h.y));
+      const uint4 q = nm::ptx::ld_shared_v4(at);
+      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
     }
   }
-  __device__ __forceinline__ void round(const F2 (&v)[4]) {   // to the storage type
+  __device__ __forceinline__ void to_shared(uint32_t at) const {
+    if constexpr (BF16) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(w[0]), "r"(w[1]) : "memory");
+    else nm::ptx::st_shared_v4(at, w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void from_global(const void* p, int64_t quad) {
     if constexpr (BF16) {
-      q[0] = make_uint4(bf16x2_of(v[0]), bf16x2_of(v[1]), bf16x2_of(v[2]), bf16x2_of(v[3]));
+      const uint2 v = __ldg(static_cast<const uint2*>(p) + quad);
+      w[0] = v.x, w[1] = v.y;
     } else {
-      float f[8];
+      const uint4 v = __ldg(static_cast<const uint4*>(p) + quad);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
+  }
+  __device__ __forceinline__ void to_global(uint8_t* p) const {
+    if constexpr (BF16) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ F2 pair(int i) const {
+    if constexpr (BF16) return f2_of(w[i]);
+    else return f2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  }
+  __device__ __forceinline__ void round(F2 a, F2 b) {   // to the storage type
+    if constexpr (BF16) {
+      w[0] = bf16x2_of(a), w[1] = bf16x2_of(b);
+    } else {
+      float f[4];
+      f2_get(a, f[0], f[1]);
+      f2_get(b, f[2], f[3]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f2_get(v[i], f[2 * i], f[2 * i + 1]);
-      q[0] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-      q[1] = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
     }
   }
 };
+
 __device__ __forceinline__ float scalar_of(const void* p, int64_t i, bool bf16) {
   return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 
-struct Gate {
-  float on, slope;   // sigmoid(g) and its derivative
-};
-__device__ __forceinline__ Gate gate_of(float g) {
-  const float e = nm::ptx::ex2_approx(-fabsf(g) * 1.4426950408889634f);
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  const float er = e * r;
-  return Gate{g >= 0.f ? r : er, er * r};   // a NaN stays one through e
-}
+// sigmoid(g) and 1 - sigmoid(g) of two gates. The exponent stops at 126: beyond it the open part is 2^-126 instead of 0,
+// and e * on stays a number (a NaN passes through).
 struct Gate2 {
-  F2 on, slope;
+  F2 on, off;
 };
+__device__ __forceinline__ float gate_exponent(float a) {
+  float r;
+  asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(r) : "f"(a));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float a) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+  return r;
+}
+__device__ __forceinline__ F2 gate_open(F2 g) {   // e = inf gives 0: no limit needed
+  float a, b;
+  f2_get(f2_mul(g, f2(-1.4426950408889634f, -1.4426950408889634f)), a, b);
+  f2_get(f2_add(f2(nm::ptx::ex2_approx(a), nm::ptx::ex2_approx(b)), f2(1.f, 1.f)), a, b);
+  return f2(rcp_approx(a), rcp_approx(b));
+}
 __device__ __forceinline__ Gate2 gate_of(F2 g) {
   float a, b;
-  f2_get(g, a, b);
-  const Gate x = gate_of(a), y = gate_of(b);
-  return Gate2{f2(x.on, y.on), f2(x.slope, y.slope)};
+  f2_get(f2_mul(g, f2(-1.4426950408889634f, -1.4426950408889634f)), a, b);
+  const F2 e = f2(nm::ptx::ex2_approx(gate_exponent(a)), nm::ptx::ex2_approx(gate_exponent(b)));
+  f2_get(f2_add(e, f2(1.f, 1.f)), a, b);
+  Gate2 r;
+  r.on = f2(rcp_approx(a), rcp_approx(b));
+  r.off = f2_mul(e, r.on);
+  return r;
 }
 
-// The value of x_out before it is rounded, two elements. `n` is the normalised branch (post) or the branch itself. Every
-// product that feeds a sum is an explicit fma or an operand of one, so forward and backward get the same bits.
+// The value of x_out before it is rounded, two elements: s x + on (n gp). A part that the call leaves out is a factor of one
+// (exact), so nothing below branches on it. Both directions use this one form and get the same bits.
 template <int GATE>
-__device__ __forceinline__ F2 outer(F2 n, F2 gp, bool post, F2 on, F2 x, F2 s, bool scaled) {
-  if constexpr (GATE == kNoGate) {
-    if (scaled) return f2_fma(s, x, post ? f2_mul(n, gp) : n);
-    return post ? f2_fma(n, gp, x) : f2_add(n, x);
-  } else {
-    const F2 y = post ? f2_mul(n, gp) : n;
-    return scaled ? f2_fma(s, x, f2_mul(on, y)) : f2_fma(on, y, x);
-  }
+__device__ __forceinline__ F2 outer(F2 n, F2 gp, F2 on, F2 x, F2 s) {
+  const F2 y = f2_mul(n, gp);
+  return f2_fma(s, x, GATE == kNoGate ? y : f2_mul(on, y));
 }
 __device__ __forceinline__ float both(F2 v) {
   float lo, hi;
@@ -122,6 +140,7 @@ struct TailParams {
   const void* dx_out; const void* da_next;
   void* dx_in; void* dbranch; void* dgate;
   float* pg_next; float* pg_post; float* pg_scale;   // [parts, D] partial sums, or nullptr
+  const void* op[5];                             // the row operands in slot order
   int64_t T, parts;
   int D, G, stages, nops;
   uint32_t op_bytes;
@@ -129,15 +148,23 @@ struct TailParams {
   uint32_t* status;
 };
 
-// Ring set-up shared by both directions; `fetch` (thread 0) brings one batch of every operand into a slot.
+template <int N>
+__device__ __forceinline__ int first_quad(const RowGroup& rg) {
+  return (rg.tg >> 5) * 32 * N + (rg.tg & 31);
+}
+
+// Ring set-up shared by both directions. A CTA owns one part, the rows [row0, row0 + rows); `fetch` (thread 0) brings the
+// batch that begins at row r of it, every operand, into a slot.
 template <bool BF16>
 struct TailRing {
   RowRing ring;
-  const uint8_t* op[5];
-  int D;
+  int D, rows;
+  int64_t row0;
   __device__ __forceinline__ void begin(uint8_t* raw, const TailParams& p, int* abort_word) {
     using namespace nm::ptx;
     D = p.D;
+    row0 = int64_t(blockIdx.x) * p.T / p.parts;
+    rows = int((int64_t(blockIdx.x) + 1) * p.T / p.parts - row0);
     ring.data = (smem_u32(raw) + 127u) & ~127u;
     ring.op_bytes = p.op_bytes, ring.stages = p.stages, ring.nops = p.nops;
     ring.full = ring.data + uint32_t(p.stages * p.nops) * p.op_bytes;
@@ -149,14 +176,21 @@ struct TailRing {
     }
     __syncthreads();
   }
-  __device__ __forceinline__ void fetch(int s, const BatchWalk& b, int groups) const {
+  __device__ __forceinline__ void fetch(const TailParams& p, int s, int r, int groups) const {
     using namespace nm::ptx;
-    const uint32_t bytes = b.rows(groups) * uint32_t(D) * (BF16 ? 2u : 4u);
+    const uint32_t bytes = uint32_t(min(groups, rows - r)) * uint32_t(D) * (BF16 ? 2u : 4u);
     const uint32_t bar = ring.full + 8u * s;
+    const int64_t at = (row0 + r) * D * (BF16 ? 2 : 4);
     mbar_arrive_expect_tx(bar, bytes * uint32_t(ring.nops));
 #pragma unroll
     for (int o = 0; o < 5; ++o)
-      if (o < ring.nops) bulk_load(ring.slot(s, o), op[o] + b.row * D * (BF16 ? 2 : 4), bytes, bar);
+      if (o < ring.nops) bulk_load(ring.slot(s, o), static_cast<const uint8_t*>(p.op[o]) + at, bytes, bar);
+  }
+  // the first stages - 1 batches; returns the row where fetching goes on
+  __device__ __forceinline__ int fill(const TailParams& p, int groups) const {
+    int r = 0;
+    for (int s = 0; s < p.stages - 1 && r < rows; ++s, r += groups) fetch(p, s, r, groups);
+    return r;
   }
 };
 
@@ -168,114 +202,106 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
   __shared__ __align__(16) float red1[2 * 8];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
+  using Q = Quad<BF16>;
+  constexpr int N = 2 * PP;
   const RowGroup rg = row_group(p.G);
-  const int D = p.D, pieces = D / 8;
+  const int quads = p.D / 4, first = first_quad<N>(rg);
   const bool post = p.g_post != nullptr, scaled = p.res_scale != nullptr;
   TailRing<BF16> tr;
-  tr.op[0] = static_cast<const uint8_t*>(p.branch);
-  tr.op[1] = static_cast<const uint8_t*>(p.x_in);
-  tr.op[2] = static_cast<const uint8_t*>(p.gate);
-  tr.op[3] = tr.op[4] = nullptr;
   tr.begin(ring_raw, p, &abort_word);
-  BatchWalk w, ahead;
-  w.begin(p.T, p.parts);
-  ahead = w;
-  if (threadIdx.x == 0)
-    for (int s = 0; s < p.stages - 1 && !ahead.done(p.parts); ++s, ahead.next(rg.groups, p.T, p.parts)) tr.fetch(s, ahead, rg.groups);
-  Raw<BF16> gn[PP], gp[PP], sc[PP];
+  int ahead = 0;
+  if (threadIdx.x == 0) ahead = tr.fill(p, rg.groups);
+  Q gn[N], gp[N], sc[N];
 #pragma unroll
-  for (int i = 0; i < PP; ++i) {
-    const int pc = rg.tg + i * rg.G;
-    gn[i].zero(), gp[i].zero(), sc[i].zero();
-    if (pc < pieces) {
-      if (p.a_next) gn[i].from_global(p.g_next, pc * 8);
-      if (post) gp[i].from_global(p.g_post, pc * 8);
-      if (scaled) sc[i].from_global(p.res_scale, pc * 8);
+  for (int j = 0; j < N; ++j) {
+    gn[j].fill(0.f), gp[j].fill(1.f), sc[j].fill(1.f);
+    if (first + 32 * j < quads) {
+      if (p.a_next) gn[j].from_global(p.g_next, first + 32 * j);
+      if (post) gp[j].from_global(p.g_post, first + 32 * j);
+      if (scaled) sc[j].from_global(p.res_scale, first + 32 * j);
     }
   }
-  const float inv_d = 1.f / float(D);
+  const float inv_d = 1.f / float(p.D);
+  auto gate_scalar = [&](int r) {
+    if constexpr (GATE == kTokenGate) return r < tr.rows ? scalar_of(p.gate, tr.row0 + r, BF16) : 0.f;
+    else return 0.f;
+  };
+  float gate_next = gate_scalar(rg.group);   // one batch ahead
   int flip = 0, flip1 = 0, s = 0;
   uint32_t phase = 0;
-  for (; !w.done(p.parts); w.next(rg.groups, p.T, p.parts)) {
-    const int64_t row = w.row + rg.group;
-    const bool on_row = row < w.end;
-    const int64_t off = row * D;
-    float tg = 0.f;
-    if constexpr (GATE == kTokenGate) tg = on_row ? gate_of(scalar_of(p.gate, row, BF16)).on : 0.f;
-    const F2 token_on = f2(tg, tg);
+  for (int r0 = rg.group; r0 < tr.rows + rg.group; r0 += rg.groups) {   // batches; this thread's row of the part is r0
+    const bool on_row = r0 < tr.rows;
+    F2 token_on = f2(1.f, 1.f);
+    if constexpr (GATE == kTokenGate) {
+      token_on = gate_open(f2(gate_next, gate_next));
+      gate_next = gate_scalar(r0 + rg.groups);
+    }
     mbar_wait<true>(tr.ring.full + 8u * s, phase, abort_flag, p.status, kErrTransformWait);
-    const uint32_t at0 = tr.ring.slot(s, 0) + uint32_t(rg.group * D + rg.tg * 8) * (BF16 ? 2u : 4u);
-    auto piece = [&](int op, int i) {
-      Raw<BF16> r;
-      r.zero();
-      if (on_row && rg.tg + i * rg.G < pieces)
-        r.from_shared(at0 + uint32_t(op) * p.op_bytes + uint32_t(i * rg.G) * uint32_t(Raw<BF16>::kBytes));
+    const uint32_t at0 = tr.ring.slot(s, 0) + uint32_t(rg.group * quads + first) * Q::kBytes;
+    auto quad = [&](int op, int j) {
+      Q r;
+      r.from_shared(at0 + uint32_t(op) * p.op_bytes + uint32_t(32 * j) * Q::kBytes);
       return r;
     };
     F2 rp = f2(1.f, 1.f);
     if (post) {   // uniform over the CTA
       F2 sbb = f2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < PP; ++i) {
-        const Raw<BF16> b = piece(0, i);
+      for (int j = 0; j < N; ++j) {
+        if (!(on_row && first + 32 * j < quads)) continue;
+        const Q b = quad(0, j);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sbb = f2_fma(b.pair(q), b.pair(q), sbb);
+        for (int q = 0; q < 2; ++q) sbb = f2_fma(b.pair(q), b.pair(q), sbb);
       }
       float sum[1] = {both(sbb)};
       group_sum<1>(sum, rg, red, flip);
       const float r = rsqrtf(fmaf(sum[0], inv_d, p.eps));
-      if (on_row && p.rstd_post && rg.tg == 0) p.rstd_post[row] = r;
+      if (on_row && p.rstd_post && rg.tg == 0) p.rstd_post[tr.row0 + r0] = r;
       rp = f2(r, r);
     }
-    Raw<BF16> xo[PP];
+    const int64_t out0 = ((tr.row0 + r0) * quads + first) * int64_t(Q::kBytes);
+    Q xo[N];
     F2 sxx = f2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < PP; ++i) {
-      const Raw<BF16> b = piece(0, i), x = piece(1, i);
-      Raw<BF16> g;
-      if constexpr (GATE == kElementGate) g = piece(2, i);
-      F2 v[4];
+    for (int j = 0; j < N; ++j) {
+      if (!(on_row && first + 32 * j < quads)) continue;
+      const Q b = quad(0, j), x = quad(1, j);
+      Q g;
+      if constexpr (GATE == kElementGate) g = quad(2, j);
+      F2 v[2];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 2; ++q) {
         F2 on = token_on;
-        if constexpr (GATE == kElementGate) on = gate_of(g.pair(q)).on;
-        const F2 n = post ? f2_mul(b.pair(q), rp) : b.pair(q);
-        v[q] = outer<GATE>(n, gp[i].pair(q), post, on, x.pair(q), sc[i].pair(q), scaled);
+        if constexpr (GATE == kElementGate) on = gate_open(g.pair(q));
+        v[q] = outer<GATE>(f2_mul(b.pair(q), rp), gp[j].pair(q), on, x.pair(q), sc[j].pair(q));
       }
-      xo[i].round(v);
-      if (on_row && rg.tg + i * rg.G < pieces) {
-        xo[i].to_global(p.x_out, off + (rg.tg + i * rg.G) * 8);
+      xo[j].round(v[0], v[1]);
+      xo[j].to_global(static_cast<uint8_t*>(p.x_out) + out0 + 32 * j * int(Q::kBytes));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sxx = f2_fma(xo[i].pair(q), xo[i].pair(q), sxx);
-      }
+      for (int q = 0; q < 2; ++q) sxx = f2_fma(xo[j].pair(q), xo[j].pair(q), sxx);
     }
     float sum[1] = {both(sxx)};
     group_sum<1>(sum, rg, red1, flip1);
-    if (threadIdx.x == 0 && !ahead.done(p.parts)) {   // the slot of the batch before takes the batch stages - 1 ahead
+    if (threadIdx.x == 0 && ahead < tr.rows) {   // the slot of the batch before takes the batch stages - 1 ahead
       const int prev = s == 0 ? p.stages - 1 : s - 1;
       mbar_wait(tr.ring.empty + 8u * prev, s == 0 ? phase ^ 1u : phase, abort_flag, p.status, kErrProducerWait);
-      tr.fetch(prev, ahead, rg.groups);
-      ahead.next(rg.groups, p.T, p.parts);
+      tr.fetch(p, prev, ahead, rg.groups);
+      ahead += rg.groups;
     }
     __syncwarp();   // the slot is not read again
     if ((threadIdx.x & 31) == 0) mbar_arrive(tr.ring.empty + 8u * s);
     if (++s == p.stages) s = 0, phase ^= 1u;
     if (on_row) {
       const float r = rsqrtf(fmaf(sum[0], inv_d, p.eps));
-      if (p.rstd_next && rg.tg == 0) p.rstd_next[row] = r;
+      if (p.rstd_next && rg.tg == 0) p.rstd_next[tr.row0 + r0] = r;
       if (p.a_next) {
         const F2 rn = f2(r, r);
 #pragma unroll
-        for (int i = 0; i < PP; ++i) {
-          const int pc = rg.tg + i * rg.G;
-          if (pc < pieces) {
-            F2 v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = f2_mul(gn[i].pair(q), f2_mul(xo[i].pair(q), rn));
-            Raw<BF16> o;
-            o.round(v);
-            o.to_global(p.a_next, off + pc * 8);
-          }
+        for (int j = 0; j < N; ++j) {
+          if (first + 32 * j >= quads) continue;
+          Q o;
+          o.round(f2_mul(gn[j].pair(0), f2_mul(xo[j].pair(0), rn)), f2_mul(gn[j].pair(1), f2_mul(xo[j].pair(1), rn)));
+          o.to_global(static_cast<uint8_t*>(p.a_next) + out0 + 32 * j * int(Q::kBytes));
         }
       }
     }
@@ -283,192 +309,216 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
   if (threadIdx.x == 0 && *abort_flag) __nanosleep(200000);   // an expired wait: let copies in flight land first
 }
 
+// The second row sum needs the first (sum(branch p) is taken over m, which needs sum(x_out a)), but m is linear in it,
+// m = h + c x_out with h = dx_out + r_n a and c = -r_n^3 sum(x_out a) / D, so
+//   sum(u m) = sum(u h) + c sum(u x_out),   u = sigmoid(gate) y,
+// and all sums are taken in the first pass, with one barrier per row. sum(branch p) = sum(u m) / r_p; for a gate per token
+// sum(m y) is the same sum without the (constant) gate. x_out as stored and h stay in registers for the second pass, the
+// gate is evaluated again; the gains lie in shared memory (of ones where the call has none). Registers decide here: beside a
+// ring that takes nearly all of the SM's memory a spilled value is read back from L2 (811 us instead of
+// TIMED us for 65536 x 2048 with both parts of the gate kept as well).
+// The gain sums of a CTA's row groups, added in group order, as one row of the partial buffer (smem: 256 float4).
+template <int N>
+__device__ __forceinline__ void write_quad_partial(const F2 (&dg)[N][2], const RowGroup& rg, int quads, float* smem, float* out_row) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int at = first_quad<N>(rg) + 32 * j;
+    float4 v;
+    f2_get(dg[j][0], v.x, v.y);
+    f2_get(dg[j][1], v.z, v.w);
+    __syncthreads();
+    reinterpret_cast<float4*>(smem)[threadIdx.x] = v;
+    __syncthreads();
+    if (rg.group == 0 && at < quads) {
+      for (int g = 1; g < rg.groups; ++g) {
+        const float4 o = reinterpret_cast<const float4*>(smem)[g * rg.G + rg.tg];
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      }
+      reinterpret_cast<float4*>(out_row)[at] = v;
+    }
+  }
+}
+
 template <bool BF16, int PP, int GATE>
 __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gated_bwd(const TailParams p) {
   using namespace nm::ptx;
   extern __shared__ __align__(128) uint8_t ring_raw[];
-  __shared__ __align__(16) float red[2 * 8];
-  __shared__ __align__(16) float red2[2 * 8 * 2];
+  __shared__ __align__(16) float red[2 * 8 * 4];
   __shared__ __align__(16) float gsm[kGroupThreads * 4];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
+  using Q = Quad<BF16>;
+  using GainQ = Quad<BF16 && PP == 4>;   // gains widened to f32 where there is room for them
+  constexpr int N = 2 * PP;
   const RowGroup rg = row_group(p.G);
-  const int D = p.D, pieces = D / 8;
-  const bool post = p.g_post != nullptr, scaled = p.res_scale != nullptr, carried = p.dx_out != nullptr;
+  const int quads = p.D / 4, first = first_quad<N>(rg);
+  const bool post = p.g_post != nullptr, carried = p.dx_out != nullptr;
   constexpr int kGateOp = 3, kCarriedOp = GATE == kElementGate ? 4 : 3;
   TailRing<BF16> tr;
-  tr.op[0] = static_cast<const uint8_t*>(p.branch);
-  tr.op[1] = static_cast<const uint8_t*>(p.x_in);
-  tr.op[2] = static_cast<const uint8_t*>(p.da_next);
-  tr.op[3] = tr.op[4] = static_cast<const uint8_t*>(p.dx_out);
-  if constexpr (GATE == kElementGate) tr.op[kGateOp] = static_cast<const uint8_t*>(p.gate);
   tr.begin(ring_raw, p, &abort_word);
-  BatchWalk w, ahead;
-  w.begin(p.T, p.parts);
-  ahead = w;
-  if (threadIdx.x == 0)
-    for (int s = 0; s < p.stages - 1 && !ahead.done(p.parts); ++s, ahead.next(rg.groups, p.T, p.parts)) tr.fetch(s, ahead, rg.groups);
-  Raw<BF16> gn[PP], gp[PP], sc[PP];
-  F2 dgn[PP][4], dgp[PP][4], dsc[PP][4];
-#pragma unroll
-  for (int i = 0; i < PP; ++i) {
-    const int pc = rg.tg + i * rg.G;
-    gn[i].zero(), gp[i].zero(), sc[i].zero();
-    if (pc < pieces) {
-      gn[i].from_global(p.g_next, pc * 8);
-      if (post) gp[i].from_global(p.g_post, pc * 8);
-      if (scaled) sc[i].from_global(p.res_scale, pc * 8);
+  int ahead = 0;
+  if (threadIdx.x == 0) ahead = tr.fill(p, rg.groups);
+  // g_next, g_post, res_scale behind the ring (ones where the call has none)
+  const uint32_t gains = (tr.ring.empty + 8u * uint32_t(p.stages) + 127u) & ~127u, gain_bytes = uint32_t(quads) * GainQ::kBytes;
+  for (int a = 0; a < 3; ++a) {
+    const void* src = a == 0 ? p.g_next : a == 1 ? p.g_post : p.res_scale;
+    for (int at = threadIdx.x; at < quads; at += kGroupThreads) {
+      Q raw;
+      raw.fill(1.f);
+      if (src) raw.from_global(src, at);
+      GainQ wide;
+      wide.round(raw.pair(0), raw.pair(1));
+      wide.to_shared(gains + uint32_t(a) * gain_bytes + uint32_t(at) * GainQ::kBytes);
     }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) dgn[i][q] = dgp[i][q] = dsc[i][q] = f2(0.f, 0.f);
   }
-  const float inv_d = 1.f / float(D);
-  int flip = 0, flip2 = 0, s = 0;
+  __syncthreads();
+  F2 dgn[N][2], dgp[N][2], dsc[N][2];
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) dgn[j][q] = dgp[j][q] = dsc[j][q] = f2(0.f, 0.f);
+  const float inv_d = 1.f / float(p.D);
+  // a row's scalars are asked for one batch ahead: every pass needs them at once
+  struct Scalars {
+    float r_n, r_p, gate;
+  };
+  auto scalars_of = [&](int r) {
+    Scalars v{0.f, 1.f, 0.f};
+    if (r < tr.rows) {
+      const int64_t row = tr.row0 + r;
+      v.r_n = __ldg(p.rstd_next + row);
+      if (post) v.r_p = __ldg(p.rstd_post + row);
+      if constexpr (GATE == kTokenGate) v.gate = scalar_of(p.gate, row, BF16);
+    }
+    return v;
+  };
+  Scalars mine = scalars_of(rg.group);
+  int flip = 0, s = 0;
   uint32_t phase = 0;
-  for (; !w.done(p.parts); w.next(rg.groups, p.T, p.parts)) {
-    const int64_t row = w.row + rg.group;
-    const bool on_row = row < w.end;
-    const int64_t off = row * D;
-    // the row's scalars are asked for before the wait, so that they land with the batch
-    const float r_n = on_row ? __ldg(p.rstd_next + row) : 0.f;
-    const float r_p = on_row && post ? __ldg(p.rstd_post + row) : 0.f;
-    Gate tgate{0.f, 0.f};
-    if constexpr (GATE == kTokenGate)
-      if (on_row) tgate = gate_of(scalar_of(p.gate, row, BF16));
-    const F2 token_on = f2(tgate.on, tgate.on), rn = f2(r_n, r_n), rp = f2(r_p, r_p);
+  for (int r0 = rg.group; r0 < tr.rows + rg.group; r0 += rg.groups) {   // batches; this thread's row of the part is r0
+    const bool on_row = r0 < tr.rows;
+    const float r_n = mine.r_n, r_p = mine.r_p;
+    Gate2 tgate{f2(1.f, 1.f), f2(0.f, 0.f)};
+    if constexpr (GATE == kTokenGate) tgate = gate_of(f2(mine.gate, mine.gate));
+    mine = scalars_of(r0 + rg.groups);
+    const F2 rn = f2(r_n, r_n), rp = f2(r_p, r_p);
     mbar_wait<true>(tr.ring.full + 8u * s, phase, abort_flag, p.status, kErrTransformWait);
-    const uint32_t at0 = tr.ring.slot(s, 0) + uint32_t(rg.group * D + rg.tg * 8) * (BF16 ? 2u : 4u);
-    auto piece = [&](int op, int i) {
-      Raw<BF16> r;
-      r.zero();
-      if (on_row && rg.tg + i * rg.G < pieces)
-        r.from_shared(at0 + uint32_t(op) * p.op_bytes + uint32_t(i * rg.G) * uint32_t(Raw<BF16>::kBytes));
+    const uint32_t at0 = tr.ring.slot(s, 0) + uint32_t(rg.group * quads + first) * Q::kBytes;
+    const uint32_t gain0 = gains + uint32_t(first) * GainQ::kBytes;
+    auto quad = [&](int op, int j) {
+      Q r;
+      r.from_shared(at0 + uint32_t(op) * p.op_bytes + uint32_t(32 * j) * Q::kBytes);
       return r;
     };
-    // x_out again, and sum(x_out a)
-    Raw<BF16> xo[PP];
-    F2 sxa = f2(0.f, 0.f);
+    auto gain = [&](int a, int j) {
+      GainQ r;
+      r.from_shared(gain0 + uint32_t(a) * gain_bytes + uint32_t(32 * j) * GainQ::kBytes);
+      return r;
+    };
+    Q xo[N];
+    F2 h[N][2];
+    F2 sxa = f2(0.f, 0.f), suh = sxa, sux = sxa;
 #pragma unroll
-    for (int i = 0; i < PP; ++i) {
-      const Raw<BF16> b = piece(0, i), x = piece(1, i), da = piece(2, i);
-      Raw<BF16> g;
-      if constexpr (GATE == kElementGate) g = piece(kGateOp, i);
-      F2 v[4];
+    for (int j = 0; j < N; ++j) {
+      if (!(on_row && first + 32 * j < quads)) continue;
+      F2 u[2], v[2];
+      {
+        Q g;
+        if constexpr (GATE == kElementGate) g = quad(kGateOp, j);
+        const Q b = quad(0, j), x = quad(1, j);
+        const GainQ gp = gain(1, j), sc = gain(2, j);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        F2 on = token_on;
-        if constexpr (GATE == kElementGate) on = gate_of(g.pair(q)).on;
-        const F2 n = post ? f2_mul(b.pair(q), rp) : b.pair(q);
-        v[q] = outer<GATE>(n, gp[i].pair(q), post, on, x.pair(q), sc[i].pair(q), scaled);
+        for (int q = 0; q < 2; ++q) {
+          F2 on = tgate.on;
+          if constexpr (GATE == kElementGate) on = gate_open(g.pair(q));
+          const F2 n = f2_mul(b.pair(q), rp);
+          v[q] = outer<GATE>(n, gp.pair(q), on, x.pair(q), sc.pair(q));
+          u[q] = f2_mul(n, gp.pair(q));
+          if constexpr (GATE == kElementGate) u[q] = f2_mul(on, u[q]);
+        }
       }
-      xo[i].round(v);
+      xo[j].round(v[0], v[1]);
+      const Q da = quad(2, j);
+      Q dxo;
+      dxo.fill(0.f);
+      if (carried) dxo = quad(kCarriedOp, j);
+      const GainQ gn = gain(0, j);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) sxa = f2_fma(xo[i].pair(q), f2_mul(gn[i].pair(q), da.pair(q)), sxa);
+      for (int q = 0; q < 2; ++q) {
+        const F2 xoq = xo[j].pair(q), a = f2_mul(gn.pair(q), da.pair(q));
+        sxa = f2_fma(xoq, a, sxa);
+        h[j][q] = f2_fma(rn, a, dxo.pair(q));
+        dgn[j][q] = f2_fma(da.pair(q), f2_mul(xoq, rn), dgn[j][q]);
+        suh = f2_fma(u[q], h[j][q], suh);
+        sux = f2_fma(u[q], xoq, sux);
+      }
     }
-    float s1[1] = {both(sxa)};
-    group_sum<1>(s1, rg, red, flip);
-    if (threadIdx.x == 0 && !ahead.done(p.parts)) {   // the slot of the batch before takes the batch stages - 1 ahead
+    float sums[3] = {both(sxa), both(suh), both(sux)};
+    group_sum<3>(sums, rg, red, flip);
+    if (threadIdx.x == 0 && ahead < tr.rows) {   // the slot of the batch before takes the batch stages - 1 ahead
       const int prev = s == 0 ? p.stages - 1 : s - 1;
       mbar_wait(tr.ring.empty + 8u * prev, s == 0 ? phase ^ 1u : phase, abort_flag, p.status, kErrProducerWait);
-      tr.fetch(prev, ahead, rg.groups);
-      ahead.next(rg.groups, p.T, p.parts);
+      tr.fetch(p, prev, ahead, rg.groups);
+      ahead += rg.groups;
     }
-    const float cn = -(r_n * r_n) * r_n * (s1[0] * inv_d);
-    const F2 c_n = f2(cn, cn);
-    F2 pv[PP][4];   // p = g_post t (post), for the last pass
-    F2 sbp = f2(0.f, 0.f), sgate = f2(0.f, 0.f);
+    const float cn = -(r_n * r_n) * r_n * (sums[0] * inv_d);
+    const float sum_um = fmaf(cn, sums[2], sums[1]);    // without the gate when it is the token's
+    float token_on, token_off, unused;
+    f2_get(tgate.on, token_on, unused);
+    f2_get(tgate.off, token_off, unused);
+    if constexpr (GATE == kTokenGate) {
+      if (on_row && rg.tg == 0) {
+        const float d = sum_um * (token_on * token_off);
+        if constexpr (BF16) static_cast<__nv_bfloat16*>(p.dgate)[tr.row0 + r0] = __float2bfloat16_rn(d);
+        else static_cast<float*>(p.dgate)[tr.row0 + r0] = d;
+      }
+    }
+    // -r_p^3 sum(branch p) / D with sum(branch p) = sum(u m) / r_p
+    const float cp = post ? -(r_p * r_p) * ((GATE == kTokenGate ? sum_um * token_on : sum_um) * inv_d) : 0.f;
+    const F2 c_n = f2(cn, cn), c_p = f2(cp, cp);
+    const int64_t out0 = ((tr.row0 + r0) * quads + first) * int64_t(Q::kBytes);
 #pragma unroll
-    for (int i = 0; i < PP; ++i) {
-      const int pc = rg.tg + i * rg.G;
-      const bool on = on_row && pc < pieces;
-      const Raw<BF16> b = piece(0, i), x = piece(1, i), da = piece(2, i);
-      Raw<BF16> g, dxo;
-      dxo.zero();
-      if constexpr (GATE == kElementGate) g = piece(kGateOp, i);
-      if (carried) dxo = piece(kCarriedOp, i);
-      F2 vx[4], vg[4], vt[4];
+    for (int j = 0; j < N; ++j) {
+      if (!(on_row && first + 32 * j < quads)) continue;
+      const Q b = quad(0, j), x = quad(1, j);
+      Q g;
+      if constexpr (GATE == kElementGate) g = quad(kGateOp, j);
+      const GainQ gp = gain(1, j), sc = gain(2, j);
+      F2 vx[2], vg[2], vb[2];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const F2 xoq = xo[i].pair(q), a = f2_mul(gn[i].pair(q), da.pair(q));
-        const F2 m = f2_fma(c_n, xoq, f2_fma(rn, a, dxo.pair(q)));
-        dgn[i][q] = f2_fma(da.pair(q), f2_mul(xoq, rn), dgn[i][q]);
-        vx[q] = scaled ? f2_mul(m, sc[i].pair(q)) : m;
-        if (scaled) dsc[i][q] = f2_fma(m, x.pair(q), dsc[i][q]);
-        const F2 n = post ? f2_mul(b.pair(q), rp) : b.pair(q);
+      for (int q = 0; q < 2; ++q) {
+        const F2 m = f2_fma(c_n, xo[j].pair(q), h[j][q]);
+        vx[q] = f2_mul(m, sc.pair(q));
+        dsc[j][q] = f2_fma(m, x.pair(q), dsc[j][q]);
+        const F2 n = f2_mul(b.pair(q), rp);
         F2 t = m;
-        if constexpr (GATE != kNoGate) {
-          const F2 my = f2_mul(m, post ? f2_mul(n, gp[i].pair(q)) : n);
-          if constexpr (GATE == kElementGate) {
-            const Gate2 z = gate_of(g.pair(q));
-            vg[q] = f2_mul(my, z.slope);
-            t = f2_mul(m, z.on);
-          } else {
-            sgate = f2_add(sgate, my);
-            t = f2_mul(m, token_on);
-          }
-        }
-        vt[q] = t;
-        if (post) {
-          dgp[i][q] = f2_fma(t, n, dgp[i][q]);
-          pv[i][q] = f2_mul(gp[i].pair(q), t);
-          sbp = f2_fma(b.pair(q), pv[i][q], sbp);
-        }
-      }
-      if (on) {
-        Raw<BF16> o;
-        o.round(vx);
-        o.to_global(p.dx_in, off + pc * 8);
+        if constexpr (GATE == kTokenGate) t = f2_mul(m, tgate.on);
         if constexpr (GATE == kElementGate) {
-          o.round(vg);
-          o.to_global(p.dgate, off + pc * 8);
+          const Gate2 z = gate_of(g.pair(q));
+          t = f2_mul(m, z.on);
+          vg[q] = f2_mul(f2_mul(t, f2_mul(n, gp.pair(q))), z.off);
         }
-        if (!post) {
-          o.round(vt);
-          o.to_global(p.dbranch, off + pc * 8);
-        }
+        dgp[j][q] = f2_fma(t, n, dgp[j][q]);
+        vb[q] = f2_fma(c_p, b.pair(q), f2_mul(rp, f2_mul(gp.pair(q), t)));
       }
-    }
-    if (post || GATE == kTokenGate) {   // uniform over the CTA
-      float s2[2] = {both(sbp), both(sgate)};
-      group_sum<2>(s2, rg, red2, flip2);
-      if constexpr (GATE == kTokenGate) {
-        if (on_row && rg.tg == 0) {
-          const float d = s2[1] * tgate.slope;
-          if constexpr (BF16) static_cast<__nv_bfloat16*>(p.dgate)[row] = __float2bfloat16_rn(d);
-          else static_cast<float*>(p.dgate)[row] = d;
-        }
-      }
-      if (post && on_row) {
-        const float cp = -(r_p * r_p) * r_p * (s2[0] * inv_d);
-        const F2 c_p = f2(cp, cp);
-#pragma unroll
-        for (int i = 0; i < PP; ++i) {
-          const int pc = rg.tg + i * rg.G;
-          if (pc < pieces) {
-            const Raw<BF16> b = piece(0, i);
-            F2 v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = f2_fma(c_p, b.pair(q), f2_mul(rp, pv[i][q]));
-            Raw<BF16> o;
-            o.round(v);
-            o.to_global(p.dbranch, off + pc * 8);
-          }
-        }
+      constexpr int kStep = 32 * int(Q::kBytes);
+      Q o;
+      o.round(vx[0], vx[1]);
+      o.to_global(static_cast<uint8_t*>(p.dx_in) + out0 + j * kStep);
+      o.round(vb[0], vb[1]);
+      o.to_global(static_cast<uint8_t*>(p.dbranch) + out0 + j * kStep);
+      if constexpr (GATE == kElementGate) {
+        o.round(vg[0], vg[1]);
+        o.to_global(static_cast<uint8_t*>(p.dgate) + out0 + j * kStep);
       }
     }
     __syncwarp();   // the warp has read all it needs of the slot
     if ((threadIdx.x & 31) == 0) mbar_arrive(tr.ring.empty + 8u * s);
     if (++s == p.stages) s = 0, phase ^= 1u;
-    if (w.last_of_part(rg.groups)) {
-      if (p.pg_next) write_gain_partial<PP>(dgn, rg, pieces, gsm, p.pg_next + int64_t(w.part) * D);
-      if (p.pg_post) write_gain_partial<PP>(dgp, rg, pieces, gsm, p.pg_post + int64_t(w.part) * D);
-      if (p.pg_scale) write_gain_partial<PP>(dsc, rg, pieces, gsm, p.pg_scale + int64_t(w.part) * D);
-#pragma unroll
-      for (int i = 0; i < PP; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) dgn[i][q] = dgp[i][q] = dsc[i][q] = f2(0.f, 0.f);
-    }
   }
+  if (p.pg_next) write_quad_partial<N>(dgn, rg, quads, gsm, p.pg_next + int64_t(blockIdx.x) * p.D);
+  if (p.pg_post) write_quad_partial<N>(dgp, rg, quads, gsm, p.pg_post + int64_t(blockIdx.x) * p.D);
+  if (p.pg_scale) write_quad_partial<N>(dsc, rg, quads, gsm, p.pg_scale + int64_t(blockIdx.x) * p.D);
   if (threadIdx.x == 0 && *abort_flag) __nanosleep(200000);   // an expired wait: let copies in flight land first
 }
 
@@ -509,13 +559,18 @@ Geometry geometry(int64_t T, int D, bool bf16, int nops, bool backward) {
   Geometry g{};
   const int pieces = D / 8;
   g.pp = pieces_per_thread_for(pieces);
+#ifdef PP1
+  if (backward) g.pp = pieces <= kGroupThreads ? 1 : pieces <= 2 * kGroupThreads ? 2 : 4;
+#endif
   g.G = group_threads_for(pieces, g.pp);
   const int groups = kGroupThreads / g.G;
-  g.ctas = g.pp <= 2 && (bf16 || !backward) ? 2 : 1;
+  g.ctas = !backward ? (g.pp <= 2 ? 2 : 1) : !bf16 ? 1 : g.pp <= 2 ? 2 : 1;
   g.op_bytes = (uint32_t(groups) * uint32_t(D) * (bf16 ? 2u : 4u) + 127u) & ~127u;
-  if (g.ctas == 2 && 2 * nops * int64_t(g.op_bytes) > 100 * 1024) g.ctas = 1;   // two stages have to fit
-  g.stages = ring_stages_for(g.ctas, nops, g.op_bytes, 4608, 6);
-  g.smem = ring_bytes(g.stages, nops, g.op_bytes);
+  const uint32_t gain_bytes = backward ? 3u * uint32_t(D) * (bf16 && g.pp == 4 ? 2u : 4u) + 128u : 0u;
+  // two stages have to fit beside the gains
+  while (g.ctas > 1 && (2 * nops * int64_t(g.op_bytes) + gain_bytes) * g.ctas > 210 * 1024) --g.ctas;
+  g.stages = ring_stages_for(g.ctas, nops, g.op_bytes, 4864 + gain_bytes, 6);
+  g.smem = ring_bytes(g.stages, nops, g.op_bytes) + gain_bytes;
   // one part per resident CTA: the fewest partial rows, and the rows are dealt evenly
   g.parts = std::min<int64_t>(std::min<int64_t>(kMaxParts, int64_t(ce::sm_count()) * g.ctas), (T + groups - 1) / groups);
   return g;
@@ -576,6 +631,7 @@ void gated_tail_fwd(bool bf16, int gate_kind, const void* branch, const void* x_
   p.branch = branch, p.x_in = x_in, p.gate = gate, p.res_scale = res_scale, p.g_post = g_post, p.g_next = g_next;
   p.x_out = x_out, p.a_next = a_next, p.rstd_post = rstd_post, p.rstd_next = rstd_next;
   p.T = T, p.D = D, p.eps = eps;
+  p.op[0] = branch, p.op[1] = x_in, p.op[2] = gate;
   launch(bf16, gate_kind, false, p, gate_kind == kElementGate ? 3 : 2, st);
 }
 
@@ -626,6 +682,8 @@ void gated_tail_bwd(bool bf16, int gate_kind, const void* dx_out, const void* da
     p.rstd_post = const_cast<float*>(rstd_post), p.rstd_next = const_cast<float*>(rstd_next);
     p.dx_out = dx_out, p.da_next = da_next, p.dx_in = dx_in, p.dbranch = dbranch, p.dgate = dgate;
     p.T = T, p.D = D;
+    const bool per_element = gate_kind == kElementGate;
+    p.op[0] = branch, p.op[1] = x_in, p.op[2] = da_next, p.op[3] = per_element ? gate : dx_out, p.op[4] = dx_out;
     launch(bf16, gate_kind, true, p, 3 + (gate_kind == kElementGate ? 1 : 0) + (dx_out ? 1 : 0), st);
   }
   if (n > 0) {
