@@ -27,6 +27,16 @@
 namespace nm::ew {
 namespace {
 
+// Two neighbouring f32 values, each operation individually rounded. Plain scalar instructions: the same kernels on the packed
+// f32x2 pipe (ew_rows.cuh) executed as many instructions and took 414 us instead of 396 us (backward, 65536 x 2048).
+struct Two {
+  float x, y;
+};
+__device__ __forceinline__ Two two(float a, float b) { return Two{a, b}; }
+__device__ __forceinline__ Two mul(Two a, Two b) { return Two{__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)}; }
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) { return Two{fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)}; }
+__device__ __forceinline__ Two two_of(uint32_t w) { return Two{lo_f32(w), hi_f32(w)}; }
+
 enum GateKind : int { kNoGate = 0, kTokenGate = 1, kElementGate = 2 };
 
 // A thread's unit is four columns: their operands are read from the slot and used at once (with eight, the operands alone
@@ -66,19 +76,15 @@ struct Quad {
     if constexpr (BF16) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  __device__ __forceinline__ F2 pair(int i) const {
-    if constexpr (BF16) return f2_of(w[i]);
-    else return f2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  __device__ __forceinline__ Two pair(int i) const {
+    if constexpr (BF16) return two_of(w[i]);
+    else return two(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
   }
-  __device__ __forceinline__ void round(F2 a, F2 b) {   // to the storage type
+  __device__ __forceinline__ void round(Two a, Two b) {   // to the storage type
     if constexpr (BF16) {
-      w[0] = bf16x2_of(a), w[1] = bf16x2_of(b);
+      w[0] = pack_bf16x2(a.x, a.y), w[1] = pack_bf16x2(b.x, b.y);
     } else {
-      float f[4];
-      f2_get(a, f[0], f[1]);
-      f2_get(b, f[2], f[3]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
+      w[0] = __float_as_uint(a.x), w[1] = __float_as_uint(a.y), w[2] = __float_as_uint(b.x), w[3] = __float_as_uint(b.y);
     }
   }
 };
@@ -90,7 +96,7 @@ __device__ __forceinline__ float scalar_of(const void* p, int64_t i, bool bf16) 
 // sigmoid(g) and 1 - sigmoid(g) of two gates. The exponent stops at 126: beyond it the open part is 2^-126 instead of 0,
 // and e * on stays a number (a NaN passes through).
 struct Gate2 {
-  F2 on, off;
+  Two on, off;
 };
 __device__ __forceinline__ float gate_exponent(float a) {
   float r;
@@ -102,35 +108,28 @@ __device__ __forceinline__ float rcp_approx(float a) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
   return r;
 }
-__device__ __forceinline__ F2 gate_open(F2 g) {   // e = inf gives 0: no limit needed
-  float a, b;
-  f2_get(f2_mul(g, f2(-1.4426950408889634f, -1.4426950408889634f)), a, b);
-  f2_get(f2_add(f2(nm::ptx::ex2_approx(a), nm::ptx::ex2_approx(b)), f2(1.f, 1.f)), a, b);
-  return f2(rcp_approx(a), rcp_approx(b));
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float gate_open(float g) {   // e = inf gives 0: no limit needed
+  return rcp_approx(__fadd_rn(1.f, nm::ptx::ex2_approx(__fmul_rn(g, -kLog2e))));
 }
-__device__ __forceinline__ Gate2 gate_of(F2 g) {
-  float a, b;
-  f2_get(f2_mul(g, f2(-1.4426950408889634f, -1.4426950408889634f)), a, b);
-  const F2 e = f2(nm::ptx::ex2_approx(gate_exponent(a)), nm::ptx::ex2_approx(gate_exponent(b)));
-  f2_get(f2_add(e, f2(1.f, 1.f)), a, b);
+__device__ __forceinline__ Two gate_open(Two g) { return two(gate_open(g.x), gate_open(g.y)); }
+__device__ __forceinline__ Gate2 gate_of(Two g) {
+  const Two e = two(nm::ptx::ex2_approx(gate_exponent(__fmul_rn(g.x, -kLog2e))),
+                    nm::ptx::ex2_approx(gate_exponent(__fmul_rn(g.y, -kLog2e))));
   Gate2 r;
-  r.on = f2(rcp_approx(a), rcp_approx(b));
-  r.off = f2_mul(e, r.on);
+  r.on = two(rcp_approx(__fadd_rn(1.f, e.x)), rcp_approx(__fadd_rn(1.f, e.y)));
+  r.off = mul(e, r.on);
   return r;
 }
 
 // The value of x_out before it is rounded, two elements: s x + on (n gp). A part that the call leaves out is a factor of one
 // (exact), so nothing below branches on it. Both directions use this one form and get the same bits.
 template <int GATE>
-__device__ __forceinline__ F2 outer(F2 n, F2 gp, F2 on, F2 x, F2 s) {
-  const F2 y = f2_mul(n, gp);
-  return f2_fma(s, x, GATE == kNoGate ? y : f2_mul(on, y));
+__device__ __forceinline__ Two outer(Two n, Two gp, Two on, Two x, Two s) {
+  const Two y = mul(n, gp);
+  return fma(s, x, GATE == kNoGate ? y : mul(on, y));
 }
-__device__ __forceinline__ float both(F2 v) {
-  float lo, hi;
-  f2_get(v, lo, hi);
-  return lo + hi;
-}
+__device__ __forceinline__ float both(Two v) { return v.x + v.y; }
 
 struct TailParams {
   const void* branch; const void* x_in; const void* gate; const void* res_scale; const void* g_post; const void* g_next;
@@ -231,9 +230,9 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
   uint32_t phase = 0;
   for (int r0 = rg.group; r0 < tr.rows + rg.group; r0 += rg.groups) {   // batches; this thread's row of the part is r0
     const bool on_row = r0 < tr.rows;
-    F2 token_on = f2(1.f, 1.f);
+    Two token_on = two(1.f, 1.f);
     if constexpr (GATE == kTokenGate) {
-      token_on = gate_open(f2(gate_next, gate_next));
+      token_on = gate_open(two(gate_next, gate_next));
       gate_next = gate_scalar(r0 + rg.groups);
     }
     mbar_wait<true>(tr.ring.full + 8u * s, phase, abort_flag, p.status, kErrTransformWait);
@@ -243,42 +242,42 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
       r.from_shared(at0 + uint32_t(op) * p.op_bytes + uint32_t(32 * j) * Q::kBytes);
       return r;
     };
-    F2 rp = f2(1.f, 1.f);
+    Two rp = two(1.f, 1.f);
     if (post) {   // uniform over the CTA
-      F2 sbb = f2(0.f, 0.f);
+      Two sbb = two(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         if (!(on_row && first + 32 * j < quads)) continue;
         const Q b = quad(0, j);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) sbb = f2_fma(b.pair(q), b.pair(q), sbb);
+        for (int q = 0; q < 2; ++q) sbb = fma(b.pair(q), b.pair(q), sbb);
       }
       float sum[1] = {both(sbb)};
       group_sum<1>(sum, rg, red, flip);
       const float r = rsqrtf(fmaf(sum[0], inv_d, p.eps));
       if (on_row && p.rstd_post && rg.tg == 0) p.rstd_post[tr.row0 + r0] = r;
-      rp = f2(r, r);
+      rp = two(r, r);
     }
     const int64_t out0 = ((tr.row0 + r0) * quads + first) * int64_t(Q::kBytes);
     Q xo[N];
-    F2 sxx = f2(0.f, 0.f);
+    Two sxx = two(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (!(on_row && first + 32 * j < quads)) continue;
       const Q b = quad(0, j), x = quad(1, j);
       Q g;
       if constexpr (GATE == kElementGate) g = quad(2, j);
-      F2 v[2];
+      Two v[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        F2 on = token_on;
+        Two on = token_on;
         if constexpr (GATE == kElementGate) on = gate_open(g.pair(q));
-        v[q] = outer<GATE>(f2_mul(b.pair(q), rp), gp[j].pair(q), on, x.pair(q), sc[j].pair(q));
+        v[q] = outer<GATE>(mul(b.pair(q), rp), gp[j].pair(q), on, x.pair(q), sc[j].pair(q));
       }
       xo[j].round(v[0], v[1]);
       xo[j].to_global(static_cast<uint8_t*>(p.x_out) + out0 + 32 * j * int(Q::kBytes));
 #pragma unroll
-      for (int q = 0; q < 2; ++q) sxx = f2_fma(xo[j].pair(q), xo[j].pair(q), sxx);
+      for (int q = 0; q < 2; ++q) sxx = fma(xo[j].pair(q), xo[j].pair(q), sxx);
     }
     float sum[1] = {both(sxx)};
     group_sum<1>(sum, rg, red1, flip1);
@@ -295,12 +294,12 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
       const float r = rsqrtf(fmaf(sum[0], inv_d, p.eps));
       if (p.rstd_next && rg.tg == 0) p.rstd_next[tr.row0 + r0] = r;
       if (p.a_next) {
-        const F2 rn = f2(r, r);
+        const Two rn = two(r, r);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           if (first + 32 * j >= quads) continue;
           Q o;
-          o.round(f2_mul(gn[j].pair(0), f2_mul(xo[j].pair(0), rn)), f2_mul(gn[j].pair(1), f2_mul(xo[j].pair(1), rn)));
+          o.round(mul(gn[j].pair(0), mul(xo[j].pair(0), rn)), mul(gn[j].pair(1), mul(xo[j].pair(1), rn)));
           o.to_global(static_cast<uint8_t*>(p.a_next) + out0 + 32 * j * int(Q::kBytes));
         }
       }
@@ -314,18 +313,19 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
 //   sum(u m) = sum(u h) + c sum(u x_out),   u = sigmoid(gate) y,
 // and all sums are taken in the first pass, with one barrier per row. sum(branch p) = sum(u m) / r_p; for a gate per token
 // sum(m y) is the same sum without the (constant) gate. x_out as stored and h stay in registers for the second pass, the
-// gate is evaluated again; the gains lie in shared memory (of ones where the call has none). Registers decide here: beside a
-// ring that takes nearly all of the SM's memory a spilled value is read back from L2 (811 us instead of
-// TIMED us for 65536 x 2048 with both parts of the gate kept as well).
+// gate is evaluated again; the gains lie in shared memory (of ones where the call has none). Beside a ring that takes
+// nearly all of the SM's memory a spilled register is read back from L2, so the registers decide the form. Measured for
+// 65536 x 2048 bf16 with a gate per element (floor 328 us at the copy rate): 811 us with the gate's two parts kept and eight
+// columns at a time (spills), 414 us as quads without spills, 396 us with scalar instead of packed f32x2 arithmetic, 353 us
+// with the next batch fetched before a batch is worked on (6.08 TB/s). Sixteen columns per thread beat eight (439 us).
 // The gain sums of a CTA's row groups, added in group order, as one row of the partial buffer (smem: 256 float4).
 template <int N>
-__device__ __forceinline__ void write_quad_partial(const F2 (&dg)[N][2], const RowGroup& rg, int quads, float* smem, float* out_row) {
+__device__ __forceinline__ void write_quad_partial(const Two (&dg)[N][2], const RowGroup& rg, int quads, float* smem, float* out_row) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int at = first_quad<N>(rg) + 32 * j;
     float4 v;
-    f2_get(dg[j][0], v.x, v.y);
-    f2_get(dg[j][1], v.z, v.w);
+    v = make_float4(dg[j][0].x, dg[j][0].y, dg[j][1].x, dg[j][1].y);
     __syncthreads();
     reinterpret_cast<float4*>(smem)[threadIdx.x] = v;
     __syncthreads();
@@ -372,11 +372,11 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
     }
   }
   __syncthreads();
-  F2 dgn[N][2], dgp[N][2], dsc[N][2];
+  Two dgn[N][2], dgp[N][2], dsc[N][2];
 #pragma unroll
   for (int j = 0; j < N; ++j)
 #pragma unroll
-    for (int q = 0; q < 2; ++q) dgn[j][q] = dgp[j][q] = dsc[j][q] = f2(0.f, 0.f);
+    for (int q = 0; q < 2; ++q) dgn[j][q] = dgp[j][q] = dsc[j][q] = two(0.f, 0.f);
   const float inv_d = 1.f / float(p.D);
   // a row's scalars are asked for one batch ahead: every pass needs them at once
   struct Scalars {
@@ -398,10 +398,16 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
   for (int r0 = rg.group; r0 < tr.rows + rg.group; r0 += rg.groups) {   // batches; this thread's row of the part is r0
     const bool on_row = r0 < tr.rows;
     const float r_n = mine.r_n, r_p = mine.r_p;
-    Gate2 tgate{f2(1.f, 1.f), f2(0.f, 0.f)};
-    if constexpr (GATE == kTokenGate) tgate = gate_of(f2(mine.gate, mine.gate));
+    Gate2 tgate{two(1.f, 1.f), two(0.f, 0.f)};
+    if constexpr (GATE == kTokenGate) tgate = gate_of(two(mine.gate, mine.gate));
     mine = scalars_of(r0 + rg.groups);
-    const F2 rn = f2(r_n, r_n), rp = f2(r_p, r_p);
+    const Two rn = two(r_n, r_n), rp = two(r_p, r_p);
+    if (threadIdx.x == 0 && ahead < tr.rows) {   // (as early as can be: two stages are all that fit) the slot of the batch before takes the batch stages - 1 ahead
+      const int prev = s == 0 ? p.stages - 1 : s - 1;
+      mbar_wait(tr.ring.empty + 8u * prev, s == 0 ? phase ^ 1u : phase, abort_flag, p.status, kErrProducerWait);
+      tr.fetch(p, prev, ahead, rg.groups);
+      ahead += rg.groups;
+    }
     mbar_wait<true>(tr.ring.full + 8u * s, phase, abort_flag, p.status, kErrTransformWait);
     const uint32_t at0 = tr.ring.slot(s, 0) + uint32_t(rg.group * quads + first) * Q::kBytes;
     const uint32_t gain0 = gains + uint32_t(first) * GainQ::kBytes;
@@ -416,12 +422,12 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
       return r;
     };
     Q xo[N];
-    F2 h[N][2];
-    F2 sxa = f2(0.f, 0.f), suh = sxa, sux = sxa;
+    Two h[N][2];
+    Two sxa = two(0.f, 0.f), suh = sxa, sux = sxa;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (!(on_row && first + 32 * j < quads)) continue;
-      F2 u[2], v[2];
+      Two u[2], v[2];
       {
         Q g;
         if constexpr (GATE == kElementGate) g = quad(kGateOp, j);
@@ -429,12 +435,12 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
         const GainQ gp = gain(1, j), sc = gain(2, j);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          F2 on = tgate.on;
+          Two on = tgate.on;
           if constexpr (GATE == kElementGate) on = gate_open(g.pair(q));
-          const F2 n = f2_mul(b.pair(q), rp);
+          const Two n = mul(b.pair(q), rp);
           v[q] = outer<GATE>(n, gp.pair(q), on, x.pair(q), sc.pair(q));
-          u[q] = f2_mul(n, gp.pair(q));
-          if constexpr (GATE == kElementGate) u[q] = f2_mul(on, u[q]);
+          u[q] = mul(n, gp.pair(q));
+          if constexpr (GATE == kElementGate) u[q] = mul(on, u[q]);
         }
       }
       xo[j].round(v[0], v[1]);
@@ -445,27 +451,19 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
       const GainQ gn = gain(0, j);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const F2 xoq = xo[j].pair(q), a = f2_mul(gn.pair(q), da.pair(q));
-        sxa = f2_fma(xoq, a, sxa);
-        h[j][q] = f2_fma(rn, a, dxo.pair(q));
-        dgn[j][q] = f2_fma(da.pair(q), f2_mul(xoq, rn), dgn[j][q]);
-        suh = f2_fma(u[q], h[j][q], suh);
-        sux = f2_fma(u[q], xoq, sux);
+        const Two xoq = xo[j].pair(q), a = mul(gn.pair(q), da.pair(q));
+        sxa = fma(xoq, a, sxa);
+        h[j][q] = fma(rn, a, dxo.pair(q));
+        dgn[j][q] = fma(da.pair(q), mul(xoq, rn), dgn[j][q]);
+        suh = fma(u[q], h[j][q], suh);
+        sux = fma(u[q], xoq, sux);
       }
     }
     float sums[3] = {both(sxa), both(suh), both(sux)};
     group_sum<3>(sums, rg, red, flip);
-    if (threadIdx.x == 0 && ahead < tr.rows) {   // the slot of the batch before takes the batch stages - 1 ahead
-      const int prev = s == 0 ? p.stages - 1 : s - 1;
-      mbar_wait(tr.ring.empty + 8u * prev, s == 0 ? phase ^ 1u : phase, abort_flag, p.status, kErrProducerWait);
-      tr.fetch(p, prev, ahead, rg.groups);
-      ahead += rg.groups;
-    }
     const float cn = -(r_n * r_n) * r_n * (sums[0] * inv_d);
     const float sum_um = fmaf(cn, sums[2], sums[1]);    // without the gate when it is the token's
-    float token_on, token_off, unused;
-    f2_get(tgate.on, token_on, unused);
-    f2_get(tgate.off, token_off, unused);
+    const float token_on = tgate.on.x, token_off = tgate.off.x;
     if constexpr (GATE == kTokenGate) {
       if (on_row && rg.tg == 0) {
         const float d = sum_um * (token_on * token_off);
@@ -475,7 +473,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
     }
     // -r_p^3 sum(branch p) / D with sum(branch p) = sum(u m) / r_p
     const float cp = post ? -(r_p * r_p) * ((GATE == kTokenGate ? sum_um * token_on : sum_um) * inv_d) : 0.f;
-    const F2 c_n = f2(cn, cn), c_p = f2(cp, cp);
+    const Two c_n = two(cn, cn), c_p = two(cp, cp);
     const int64_t out0 = ((tr.row0 + r0) * quads + first) * int64_t(Q::kBytes);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -484,22 +482,24 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
       Q g;
       if constexpr (GATE == kElementGate) g = quad(kGateOp, j);
       const GainQ gp = gain(1, j), sc = gain(2, j);
-      F2 vx[2], vg[2], vb[2];
+      Two vx[2], vg[2], vb[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const F2 m = f2_fma(c_n, xo[j].pair(q), h[j][q]);
-        vx[q] = f2_mul(m, sc.pair(q));
-        dsc[j][q] = f2_fma(m, x.pair(q), dsc[j][q]);
-        const F2 n = f2_mul(b.pair(q), rp);
-        F2 t = m;
-        if constexpr (GATE == kTokenGate) t = f2_mul(m, tgate.on);
+        const Two m = fma(c_n, xo[j].pair(q), h[j][q]);
+        vx[q] = mul(m, sc.pair(q));
+        dsc[j][q] = fma(m, x.pair(q), dsc[j][q]);
+        Two t = mul(m, rp);   // t r_p from here on: its products with the branch are those of t with the normalised branch
+        if constexpr (GATE == kTokenGate) t = mul(t, tgate.on);
+        Two off;
         if constexpr (GATE == kElementGate) {
           const Gate2 z = gate_of(g.pair(q));
-          t = f2_mul(m, z.on);
-          vg[q] = f2_mul(f2_mul(t, f2_mul(n, gp.pair(q))), z.off);
+          t = mul(t, z.on);
+          off = z.off;
         }
-        dgp[j][q] = f2_fma(t, n, dgp[j][q]);
-        vb[q] = f2_fma(c_p, b.pair(q), f2_mul(rp, f2_mul(gp.pair(q), t)));
+        dgp[j][q] = fma(t, b.pair(q), dgp[j][q]);
+        const Two pr = mul(gp.pair(q), t);
+        if constexpr (GATE == kElementGate) vg[q] = mul(mul(pr, b.pair(q)), off);
+        vb[q] = fma(c_p, b.pair(q), pr);
       }
       constexpr int kStep = 32 * int(Q::kBytes);
       Q o;
@@ -559,9 +559,6 @@ Geometry geometry(int64_t T, int D, bool bf16, int nops, bool backward) {
   Geometry g{};
   const int pieces = D / 8;
   g.pp = pieces_per_thread_for(pieces);
-#ifdef PP1
-  if (backward) g.pp = pieces <= kGroupThreads ? 1 : pieces <= 2 * kGroupThreads ? 2 : 4;
-#endif
   g.G = group_threads_for(pieces, g.pp);
   const int groups = kGroupThreads / g.G;
   g.ctas = !backward ? (g.pp <= 2 ? 2 : 1) : !bf16 ? 1 : g.pp <= 2 ? 2 : 1;
