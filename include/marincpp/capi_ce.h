@@ -143,6 +143,24 @@ int nm_ce_sampled_head(int rounding, int logits_store, const void* x, const void
                        int32_t* n_candidates_out, void* workspace, void* stream, float z_loss_weight,
                        int32_t ignore_index);
 
+/* ---- distillation head (C++, with the formulas: include/marincpp/kernels/distill_head.hpp): per row the loss
+ *        soft_weight tau^2 KL(q || softmax(z / tau)) + hard_weight (lse(z) - z[target]),   z = x W^T,
+ *      against a teacher's listed logits [T, K] (ids outside [0, V) are padding), q their softmax at temperature tau, or with
+ *      teacher_lse [T] (log sum exp(. / tau) over the teacher's whole vocabulary) their true masses; and its gradients
+ *      dx [T, D] bf16 (accumulate_dx: added to) and dw [V, D] f32 (added to). x, w bf16, D % 8 == 0; teacher_dtype 0 f32,
+ *      1 bf16; K 1 .. 512. NULL: teacher_lse, targets (when hard_weight is 0), kl_tok, lse (log sum exp(z / tau)),
+ *      loss_partial, dx, dw, and grad_scale when both are NULL. dx may be x when it does not accumulate. forward_only != 0:
+ *      no gradients, and a workspace without a logits store. Same bits for the same call and chunk_rows. workspace: 256-byte
+ *      aligned, nm_ce_distill_workspace_bytes (0 on error) with the same arguments; word 0 is the wait status
+ *      (nm_ce_device_status). Nothing is allocated; the call can be captured into a CUDA graph (make the first call on a
+ *      device outside a capture). --------------------------------------------------------------------------------- */
+uint64_t nm_ce_distill_workspace_bytes(int64_t T, int D, int V, int K, int chunk_rows, int forward_only);
+int nm_ce_distill(int teacher_dtype, const void* x, const void* w, const int32_t* teacher_ids, const void* teacher_logits,
+                  const float* teacher_lse, const int32_t* targets, const float* weight, const float* grad_scale,
+                  float temperature, float soft_weight, float hard_weight, float* loss_tok, float* kl_tok, float* lse,
+                  float* loss_partial, void* dx, int accumulate_dx, float* dw, int forward_only, int64_t T, int D, int V, int K,
+                  int chunk_rows, int32_t ignore_index, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- data-parallel dW reduction over NCCL (the role of the reference's include/marincpp/comm.hpp:22-58 GradReducer
  *      and of src/train/trainer.cpp:50,139): one communicator per process (one process per GPU) ------------------- */
 int nm_comm_unique_id(void* id128_host);                       /* rank 0: 128 bytes to broadcast to the other ranks */

@@ -40,14 +40,21 @@ __host__ __device__ constexpr int num_stages(int ncta) { return ncta == 2 ? 6 : 
 // logits epilogue adds 1 KiB where the two column halves of a row meet to merge their (max, sum exp)
 constexpr int kMergeBytes = BM * 8;
 __host__ __device__ constexpr int epi_stage_bytes(int epi) {
-  return (epi == kEpiLogits || epi == kEpiDw) ? kEpiWarps * kEpiBufBytes + (epi == kEpiLogits ? kMergeBytes : 0) : 0;
+  return (epi == kEpiLogits || epi == kEpiDw)
+             ? kEpiWarps * kEpiBufBytes + (epi == kEpiLogits ? kMergeBytes : 0)
+             : epi == kEpiDistill ? kEpiWarps * kEpiBufBytes + BM * 12 : 0;   // (max, two sums) per row
 }
 constexpr int smem_bytes(int epi, int ncta) {
   return num_stages(ncta) * stage_bytes(ncta) + epi_stage_bytes(epi) + 1024 /*alignment slack*/ + 256 /*barriers*/;
 }
 
 // ---------------------------------------------------------------------------------------------- the kernel
-template <int EPI, bool A_MN, bool B_MN, int NCTA>
+// TWO (the distillation head's gradient contractions): A is the two-term gradient of ce_internal.hpp. dX (A K-major): K
+// block kb is the hi block kb, at column 128 kb; the tiles are dealt k_parts times, each time over its own k_part K blocks.
+// dW (A MN-major): K blocks alternate between the terms of the same 64 rows; a CTA takes its tile k_parts times in a row,
+// k_part K blocks each, and its epilogue lets the additions of one part finish before it issues those of the next, so that
+// the order of additions is fixed.
+template <int EPI, bool A_MN, bool B_MN, int NCTA, bool TWO = false>
 __global__ void __launch_bounds__(kThreads, 1)
 k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
           const __grid_constant__ CUtensorMap tmC, const GemmParams p) {
@@ -101,9 +108,21 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  const int num_tiles = p.num_m * p.num_n;
-  const int k_blocks = (p.K + BK - 1) / BK;
+  const int num_tiles = TWO && !A_MN ? p.num_m * p.num_n * p.k_parts : p.num_m * p.num_n;
+  const int all_k_blocks = (p.K + BK - 1) / BK * (TWO && A_MN ? 2 : 1);
+  const int parts = TWO && A_MN ? p.k_parts : 1;            // passes of a CTA over its tile
+  // K blocks [kb0, kb1) of pass `part` over `tile`
+  auto k_range = [&](int tile, int part, int& kb0, int& kb1) {
+    if constexpr (TWO) {
+      const int share = A_MN ? part : tile / (p.num_m * p.num_n);
+      kb0 = share * p.k_part;
+      kb1 = min(kb0 + p.k_part, all_k_blocks);
+    } else {
+      kb0 = 0, kb1 = all_k_blocks;
+    }
+  };
   auto decode = [&](int tile, int& mi, int& ni) {
+    if constexpr (TWO && !A_MN) tile %= p.num_m * p.num_n;
     if (p.m_inner) {
       const int per_group = p.m_group * p.num_n;
       const int g = tile / per_group, r = tile - g * per_group;
@@ -123,7 +142,7 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
       bool ok = true;
       // L2 eviction hints, fixed per kernel: the logits kernel re-reads the x rows of a tile group for every
       // vocabulary tile and the dW kernel re-reads the whole x chunk for every vocabulary tile (keep: evict last)
-      constexpr int kAPol = EPI == kEpiLogits ? 2 : 0;
+      constexpr int kAPol = EPI == kEpiLogits || EPI == kEpiDistill ? 2 : 0;
       constexpr int kBPol = EPI == kEpiDw ? 2 : 0;
       const uint64_t pol_last = l2_policy_evict_last();
       // pair mode: the bytes of both CTAs are counted on the leader's barrier, which only the leader arms
@@ -152,13 +171,20 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         int mi, ni;
         decode(tile, mi, ni);
         const int m0 = p.m_off + mi * BMT + int(rank) * BM, n0 = ni * BN + int(rank) * BNC;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        int kb0, kb1;
+        k_range(tile, 0, kb0, kb1);
+        if constexpr (TWO && A_MN) kb1 = all_k_blocks;       // the passes follow one another
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait<true>(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kErrProducerWait)) { ok = false; break; }
           const uint32_t bar = NCTA == 2 ? mapa_shared(full_bar(stage), 0) : full_bar(stage);
           if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), NCTA * kStageBytes);
           const uint32_t a_dst = sA + stage * kABytes, b_dst = sB + stage * kBBytes;
-          const int k0 = kb * BK;
-          if constexpr (A_MN) {
+          const int k0 = (TWO && A_MN ? kb >> 1 : kb) * BK;
+          if constexpr (TWO && A_MN) {
+            tma_load_4d(a_dst, &tmA, bar, 0, k0, kb & 1, m0 >> 6);
+          } else if constexpr (TWO) {
+            ld2(a_dst, &tmA, bar, 2 * k0, m0, keepA);
+          } else if constexpr (A_MN) {
             if (p.a_3d) {
               ld3(a_dst, &tmA, bar, 0, k0, m0 >> 6, keepA);
             } else {
@@ -189,12 +215,15 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
       int stage = 0; uint32_t phase = 0;
       int it = 0;
       bool ok = true;
-      for (int tile = walker; tile < num_tiles && ok; tile += walkers, ++it) {
+      for (int tile = walker, part = 0; tile < num_tiles && ok; ++it) {
         const int b = it & 1;
+        int kb0, kb1;
+        k_range(tile, part, kb0, kb1);
+        if (++part >= parts) part = 0, tile += walkers;
         if (!mbar_wait(tempty_bar(b), ((it >> 1) & 1u) ^ 1u, abort_flag, p.status, kErrTmemFreeWait)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + uint32_t(b * BN);
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kErrMmaWait)) { ok = false; break; }
           tc_fence_after();
           const uint32_t a_src = sA + stage * kABytes, b_src = sB + stage * kBBytes;
@@ -205,8 +234,8 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
                                      : smem_desc_sw128(a_src + k * (UK * 2), 16, 1024);
             const uint64_t bd = B_MN ? smem_desc_sw128(b_src + k * (UK * 128), kBoxBytesMN, 1024)
                                      : smem_desc_sw128(b_src + k * (UK * 2), 16, 1024);
-            if constexpr (NCTA == 2) umma_pair_bf16(d_tmem, ad, bd, idesc, (kb | k) != 0);
-            else umma_bf16(d_tmem, ad, bd, idesc, (kb | k) != 0);
+            if constexpr (NCTA == 2) umma_pair_bf16(d_tmem, ad, bd, idesc, kb != kb0 || k != 0);
+            else umma_bf16(d_tmem, ad, bd, idesc, kb != kb0 || k != 0);
           }
           // the stage is free again once these UMMAs have read it (pair mode: in both CTAs)
           if constexpr (NCTA == 2) umma_pair_commit(empty_bar(stage), 3);
@@ -233,10 +262,11 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     const uint64_t store_policy = l2_policy_evict_first();   // the logits store is not read again by this kernel
     constexpr int kChunks = BN / 32 / 2;       // 32-column chunks per warp
     int it = 0;
-    for (int tile = walker; tile < num_tiles; tile += walkers, ++it) {
-      const int b = it & 1;
+    for (int tile_at = walker, part = 0; tile_at < num_tiles; ++it) {
+      const int b = it & 1, tile = tile_at;
       int mi, ni;
       decode(tile, mi, ni);
+      if (++part >= parts) part = 0, tile_at += walkers;
       const int m0 = mi * BMT + int(rank) * BM, n0 = ni * BN;
       const int grow = m0 + r_local;
       const bool row_ok = grow < p.M;
@@ -245,8 +275,14 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
       tc_fence_after();
       const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(b * BN + half * (BN / 2));
       LogitsRowState st{-INFINITY, 0.f, 0.f, false};
+      DistillRowState ds{-INFINITY, 0.f, 0.f, 0.f, false};
       int tg = -1;
       if constexpr (EPI == kEpiLogits) tg = row_ok ? __ldg(p.targets + grow) : -1;
+      if constexpr (EPI == kEpiDistill) tg = row_ok && p.targets ? __ldg(p.targets + grow) : -1;
+      if constexpr (TWO && EPI == kEpiDw) {
+        if (lane == 0) bulk_wait<0>();         // the additions of the pass before have been performed
+        __syncwarp();
+      }
 
       // one 32-column chunk held in v[]; c counts the chunks of the whole tile (0 .. 7)
       auto process = [&](float* v, int c) {
@@ -268,6 +304,29 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
               bulk_commit();
             }
             ++n_bulk;
+          }
+        } else if constexpr (EPI == kEpiDistill) {
+          epi_distill_chunk(p, v, col0, tg, ds);
+          if (p.store != nullptr && warp_rows_ok) {
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
+            stage_f32_row(stg, lane, v, 1.f, false);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {                   // rows and columns beyond the matrix are clipped by the tensor map
+              tma_store_2d_hint(&tmC, stg, col0, m0 + quad * 32, store_policy);
+              bulk_commit();
+            }
+          }
+        } else if constexpr (TWO && EPI == kEpiDx) {
+          if (row_ok && p.c) {                 // one share of a split contraction: the f32 sums as they are
+            float* o = p.c + (int64_t(tile / (p.num_m * p.num_n)) * p.M + grow) * p.ldc + col0;
+            const int ncols = min(32, p.N - col0);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              if (j < ncols) *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          } else if (row_ok) {
+            epi_dx_chunk(p, v, grow, col0, scale);
           }
         } else if constexpr (EPI == kEpiDx) {
           if (row_ok) epi_dx_chunk(p, v, grow, col0, scale);
@@ -342,6 +401,31 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
           }
         }
       }
+      if constexpr (EPI == kEpiDistill) {      // the same hand-over with two sums
+        float* dm = reinterpret_cast<float*>(merge);
+        if (ds.hit) p.zt[grow] = ds.zt;
+        const uint32_t mphase = uint32_t(it) & 1u;
+        if (half == 1) {
+          if (!mbar_wait<true>(mempty_bar(quad), mphase ^ 1u, abort_flag, p.status, kErrEpilogueWait)) break;
+          dm[r_local] = ds.m, dm[BM + r_local] = ds.s, dm[2 * BM + r_local] = ds.s1;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(mfull_bar(quad));
+        } else {
+          if (!mbar_wait<true>(mfull_bar(quad), mphase, abort_flag, p.status, kErrEpilogueWait)) break;
+          const float om = dm[r_local], os = dm[BM + r_local], os1 = dm[2 * BM + r_local];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(mempty_bar(quad));
+          constexpr float kLog2e = 1.4426950408889634f;
+          const float m = fmaxf(ds.m, om), c = p.tau_log2e;   // ds.m is finite: the left half holds a valid column
+          if (row_ok) {
+            const int64_t at = int64_t(ni) * p.ldT + grow;
+            p.tmax[at] = m;
+            p.tsum[at] = ds.s * ex2_approx(fmaf(ds.m, c, -m * c)) + os * ex2_approx(fmaf(om, c, -m * c));
+            if (p.tsum1)
+              p.tsum1[at] = ds.s1 * ex2_approx(fmaf(ds.m, kLog2e, -m * kLog2e)) + os1 * ex2_approx(fmaf(om, kLog2e, -m * kLog2e));
+          }
+        }
+      }
     }
     if constexpr (epi_stage_bytes(EPI) > 0) {
       if (lane == 0) bulk_wait<0>();           // every staged store / reduction has been performed
@@ -389,14 +473,14 @@ __global__ void __launch_bounds__(64) k_wait_timeout_probe(uint32_t* status, lon
 }
 
 
-template <int EPI, bool A_MN, bool B_MN, int NCTA>
+template <int EPI, bool A_MN, bool B_MN, int NCTA, bool TWO = false>
 void launch_n(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const GemmParams& p,
               cudaStream_t st, int sm_reserve) {
-  auto kernel = k_ce_umma<EPI, A_MN, B_MN, NCTA>;
+  auto kernel = k_ce_umma<EPI, A_MN, B_MN, NCTA, TWO>;
   constexpr int kSmem = smem_bytes(EPI, NCTA);
   static_assert(kSmem <= 232448, "dynamic shared memory beyond the 227 KiB a CTA may use");
   NM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-  const int tiles = p.num_m * p.num_n;
+  const int tiles = p.num_m * p.num_n * (TWO && !A_MN ? p.k_parts : 1);
   const int walkers = std::max(1, (sm_count() - std::max(0, sm_reserve)) / NCTA);   // CTAs, or pairs of CTAs
   const int grid = NCTA * std::min(tiles, walkers);
   cudaLaunchConfig_t cfg{};
@@ -495,6 +579,71 @@ void launch_wgrad(const WgradArgs& a, cudaStream_t st) {
   const CUtensorMap tb = tmap_mn_b(a.x, a.rows, a.D, a.ldx, p.b_3d, ncta);
   const CUtensorMap tc = tmap_epilogue(a.dw, a.V, a.D, a.D, true);
   launch<kEpiDw, true, true>(ncta, ta, tb, tc, p, st, a.sm_reserve);
+}
+
+void launch_distill_logits(const DistillLogitsArgs& a, cudaStream_t st) {
+  if (a.rows <= 0) return;
+  GemmParams p{};
+  const int ncta = ncta_for(0, a.rows, a.D), bmt = BM * ncta;
+  p.M = a.rows; p.N = a.V; p.K = a.D;
+  p.num_m = (a.rows + bmt - 1) / bmt; p.num_n = (a.V + BN - 1) / BN; p.m_inner = 1;
+  p.m_group = int(std::max<int64_t>(1, std::min<int64_t>(p.num_m, (int64_t(16) << 20) / (int64_t(bmt) * a.D * 2))));
+  p.status = a.status;
+  p.store = a.store; p.ldS = a.ldS; p.store_f32 = 1;
+  p.tmax = a.tmax; p.tsum = a.tsum; p.tsum1 = a.tsum1; p.ldT = a.ldT; p.zt = a.zt; p.targets = a.targets;
+  p.tau_log2e = 1.4426950408889634f / a.tau;
+  const CUtensorMap ta = tmap_kmajor(a.x, a.rows, a.D, a.D, BM);
+  const CUtensorMap tb = tmap_kmajor(a.w, a.V, a.D, a.D, BN / ncta);
+  const CUtensorMap tc = a.store ? tmap_epilogue(a.store, a.rows, a.V, a.ldS, true) : ta;
+  launch<kEpiDistill, false, false>(ncta, ta, tb, tc, p, st);
+}
+
+// Shares of the dX contraction: one CTA per tile leaves SMs idle when a call has few tiles, or a last wave with few of them.
+// Of up to 16 shares the one with the fewest K blocks per SM is taken, a share counting 24 blocks more for its epilogue
+// and the reading of its sums; the sums take at most 32768 x D f32.
+int distill_dgrad_shares(int rows, int D, int V) {
+  const int64_t tiles = int64_t((rows + BM - 1) / BM) * ((D + BN - 1) / BN), kb = (V + BK - 1) / BK, sms = sm_count();
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= 16 && int64_t(s) * rows <= 32768 && s <= kb; ++s) {
+    const int64_t per = (kb + s - 1) / s;
+    if ((kb + per - 1) / per != s) continue;   // a share would be empty
+    const int64_t cost = (tiles * s + sms - 1) / sms * (per + (s > 1 ? 24 : 0));
+    if (cost < least) least = cost, best = s;
+  }
+  return best;
+}
+
+void launch_distill_dgrad(const DistillDgradArgs& a, cudaStream_t st) {
+  if (a.rows <= 0) return;
+  GemmParams p{};
+  p.M = a.rows; p.N = a.D; p.K = a.V;
+  p.num_m = (a.rows + BM - 1) / BM; p.num_n = (a.D + BN - 1) / BN; p.m_group = 1;
+  p.status = a.status;
+  p.scale = a.scale; p.dx_old = a.dx_old; p.dx_out = a.dx_out; p.acc_mode = a.dx_old ? a.acc_mode : 0; p.ldo = a.D;
+  p.c = a.shares > 1 ? a.part : nullptr; p.ldc = a.D;
+  const int kb = (a.V + BK - 1) / BK;
+  p.k_part = (kb + a.shares - 1) / a.shares;
+  p.k_parts = a.shares;
+  NM_REQUIRE((p.k_parts - 1) * p.k_part < kb, "distillation: an empty share of the dX contraction");
+  const CUtensorMap ta = tmap_kmajor(a.n, a.rows, a.ldn, a.ldn, BM);   // spans both terms
+  const CUtensorMap tb = tmap_mn_b(a.w, a.V, a.D, a.D, p.b_3d, 1);
+  launch_n<kEpiDx, false, true, 1, true>(ta, tb, ta, p, st, 0);
+}
+
+void launch_distill_wgrad(const DistillWgradArgs& a, cudaStream_t st) {
+  if (a.rows <= 0) return;
+  GemmParams p{};
+  p.M = a.V; p.N = a.D; p.K = a.rows;
+  p.num_m = (a.V + BM - 1) / BM; p.num_n = (a.D + BN - 1) / BN; p.m_group = 1;
+  p.status = a.status;
+  p.scale = a.scale; p.dw = a.dw;
+  p.k_part = 2 * kDrainRows / BK;
+  p.k_parts = (a.rows + kDrainRows - 1) / kDrainRows;
+  const CUtensorMap ta = tmap_two_term_mn_a(a.n, a.rows, a.ldn);
+  const CUtensorMap tb = tmap_mn_b(a.x, a.rows, a.D, a.D, p.b_3d, 1);
+  const CUtensorMap tc = tmap_epilogue(a.dw, a.V, a.D, a.D, true);
+  launch_n<kEpiDw, true, true, 1, true>(ta, tb, tc, p, st, 0);
 }
 
 void set_cta_pair(int logits, int dgrad, int wgrad) {

@@ -153,6 +153,45 @@ struct WgradArgs {
 };
 void launch_wgrad(const WgradArgs& a, cudaStream_t st);
 
+// ---- the distillation head's contractions (ce_gemm.cu), on the same template
+// z = x W^T: the f32 logits (store [rows, ldS] or nullptr), per 256-column tile max z, sum exp((z - max) / tau) and (tsum1 or
+// nullptr) sum exp(z - max); z[target] -> zt for targets inside [0, V) (targets may be nullptr).
+struct DistillLogitsArgs {
+  const void* x; const void* w; const int32_t* targets;
+  int rows, D, V;
+  float tau;
+  float* store; int64_t ldS;
+  float* tmax; float* tsum; float* tsum1; int64_t ldT;
+  float* zt;
+  uint32_t* status;
+};
+void launch_distill_logits(const DistillLogitsArgs& a, cudaStream_t st);
+
+// The gradient n as two bf16 terms, hi + lo, in blocks of 64 columns: block b of hi at columns [128 b, 128 b + 64), of lo
+// behind it (row pitch ldn bf16 elements, a multiple of 128).
+//   dX: shares of the contraction over V are summed apart (part [shares, rows, D] f32, added up by the caller) when shares
+//       > 1; else the epilogue writes dx as DgradArgs does. Only hi is contracted: dx is stored in bf16.
+//   dW: both terms; the accumulator is drained into dw (f32) after every kDrainRows rows, because the tensor core adds to it
+//       with truncation (measured: the relative error of a contraction of length K grows as 1e-9 K).
+constexpr int kDrainRows = 1024;
+struct DistillDgradArgs {
+  const void* n; int64_t ldn; const void* w;
+  int rows, D, V;
+  const float* scale;
+  const void* dx_old; void* dx_out; int acc_mode;
+  float* part; int shares;
+  uint32_t* status;
+};
+int distill_dgrad_shares(int rows, int D, int V);   // how many shares pay on the current device
+void launch_distill_dgrad(const DistillDgradArgs& a, cudaStream_t st);
+struct DistillWgradArgs {
+  const void* n; int64_t ldn; const void* x;
+  int rows, D, V;
+  const float* scale; float* dw;
+  uint32_t* status;
+};
+void launch_distill_wgrad(const DistillWgradArgs& a, cudaStream_t st);
+
 // unit-test entry: one CTA whose bounded wait runs out after `limit_cycles` (<= 2e6) on a barrier nobody completes
 void launch_wait_timeout_probe(uint32_t* status, long long limit_cycles, int* saw_abort, cudaStream_t st);
 

@@ -24,7 +24,7 @@ constexpr int kBoxBytesMN = 64 * BK * 2;        // one MN-major box: 64 k-rows o
 constexpr int kTmemCols = 512;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-enum Epi : int { kEpiLogits = 0, kEpiDx = 1, kEpiDw = 2, kEpiTest = 3 };
+enum Epi : int { kEpiLogits = 0, kEpiDx = 1, kEpiDw = 2, kEpiTest = 3, kEpiDistill = 4 };
 constexpr int kEpiBufBytes = 32 * 128;          // one 32-row x 128-byte staging tile per epilogue warp
 
 struct GemmParams {
@@ -48,6 +48,11 @@ struct GemmParams {
   float* c; int64_t ldc;
   // gradient kernels that form n on the fly: per-row factors, indexed by the row of the logits store
   const RowFactors* rowf;
+  // distillation: log2e / temperature, and sum exp(z - max) at temperature 1 (nullptr: not wanted)
+  float tau_log2e; float* tsum1;
+  // contractions over a gradient held as two bf16 terms: K blocks per pass over the tile (segments drained one by one, dW)
+  // and per share of a split contraction (dX), and the number of either
+  int k_part, k_parts;
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -124,6 +129,48 @@ __device__ __forceinline__ void epi_logits_chunk(const GemmParams& p, float* v, 
   // st.m == -inf on the first chunk: ex2(-inf) = 0 and st.s = 0
   st.s = st.s * ex2_approx(fmaf(st.m, kLog2e, neg)) + ((a0 + a1) + (a2 + a3));
   st.m = m_new;
+  if (tg >= col0 && tg < col0 + 32) {
+    const int jt = tg - col0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j == jt) st.zt = v[j];
+    st.hit = true;
+  }
+}
+
+// The distillation head's statistics: the maximum of the raw logits, sum exp((z - max) / tau) and, when wanted, sum
+// exp(z - max), online as above. The f32 logits leave through the staging tile (the caller).
+struct DistillRowState {
+  float m, s, s1, zt;
+  bool hit;
+};
+__device__ __forceinline__ void epi_distill_chunk(const GemmParams& p, const float* v, int col0, int tg, DistillRowState& st) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  const int ncols = min(32, p.N - col0);
+  const bool whole = ncols == 32;
+  float cm = v[0];                          // the first column of a chunk exists
+#pragma unroll
+  for (int j = 1; j < 32; ++j)
+    if (whole || j < ncols) cm = fmaxf(cm, v[j]);
+  const float m = fmaxf(st.m, cm), c = p.tau_log2e, neg = -m * c;
+  float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    if (whole || j < ncols) a0 += ex2_approx(fmaf(v[j], c, neg));
+    if (whole || j + 1 < ncols) a1 += ex2_approx(fmaf(v[j + 1], c, neg));
+  }
+  st.s = st.s * ex2_approx(fmaf(st.m, c, neg)) + (a0 + a1);   // st.m == -inf on the first chunk: ex2(-inf) = 0
+  if (p.tsum1) {                            // uniform over the launch
+    const float neg1 = -m * kLog2e;
+    float b0 = 0.f, b1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      if (whole || j < ncols) b0 += ex2_approx(fmaf(v[j], kLog2e, neg1));
+      if (whole || j + 1 < ncols) b1 += ex2_approx(fmaf(v[j + 1], kLog2e, neg1));
+    }
+    st.s1 = st.s1 * ex2_approx(fmaf(st.m, kLog2e, neg1)) + (b0 + b1);
+  }
+  st.m = m;
   if (tg >= col0 && tg < col0 + 32) {
     const int jt = tg - col0;
 #pragma unroll
@@ -279,6 +326,24 @@ inline CUtensorMap tmap_mn_a(const void* base, int64_t K, int64_t MN, int64_t ld
 inline CUtensorMap tmap_mn_b(const void* base, int64_t K, int64_t MN, int64_t ld, int& is3d, int ncta) {
   is3d = MN % 64 == 0;
   return is3d ? tmap_mnmajor_3d(base, K, MN, ld, BN / ncta / 64) : tmap_mnmajor(base, K, MN, ld);
+}
+
+// The gradient as two bf16 terms, blocks of 64 columns of the first term and of the second in turn (row pitch ldn bf16
+// elements, a multiple of 128): as the MN-major A operand of dW, a 4-D tensor (64 columns, rows, term, column block) whose
+// box (64, 64 rows, one term, BM / 64 blocks) lands like that of the 3-D map.
+inline CUtensorMap tmap_two_term_mn_a(const void* base, int64_t rows, int64_t ldn) {
+  NM_REQUIRE(ldn % 128 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0, "distillation: two-term operand alignment");
+  CUtensorMap m;
+  const cuuint64_t dims[4] = {64, cuuint64_t(rows), 2, cuuint64_t(ldn / 128)};
+  const cuuint64_t strides[3] = {cuuint64_t(ldn) * 2, 128, 256};
+  const cuuint32_t box[4] = {64, BK, 1, BM / 64};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    throw DeviceError("distillation: cuTensorMapEncodeTiled (4-D) failed with CUresult " + std::to_string(int(r)));
+  return m;
 }
 
 // epilogue staging tile as a tensor-map box: 32 rows x 32 columns (f32: 128-byte rows, SWIZZLE_128B; bf16: 64-byte

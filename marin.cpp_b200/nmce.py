@@ -65,6 +65,9 @@ SIGS = {
     "nm_gated_tail_workspace_bytes": (U64, [I64, I32]),
     "nm_gated_tail_bwd": (I32, [I32, I32, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, VP, I64, I32, VP, U64,
                                 VP]),
+    "nm_ce_distill_workspace_bytes": (U64, [I64, I32, I32, I32, I32, I32]),
+    "nm_ce_distill": (I32, [I32, VP, VP, VP, VP, VP, VP, VP, VP, F32, F32, F32, VP, VP, VP, VP, VP, I32, VP, I32, I64, I32,
+                            I32, I32, I32, C.c_int32, VP, U64, VP]),
     "nm_comm_unique_id": (I32, [VP]),
     "nm_comm_create": (I32, [VP, I32, I32, VP]),
     "nm_comm_destroy": (I32, [VP]),
@@ -94,7 +97,8 @@ SIGS = {
 }
 NO_STATUS = {"nm_version", "nm_last_error", "nm_device_arch", "nm_ce_workspace_bytes", "nm_ce_set_backends",
              "nm_ce_device_arch", "nm_ce_set_fast_stats_exp", "nm_ce_sampled_stride", "nm_ce_sampled_workspace_bytes", "nm_norm_partial_rows", "nm_head_adamh_owned_elems", "nm_grad_reducer_owned_elems", "nm_ce_suggest_chunk_rows",
-             "nm_embed_bwd_workspace_bytes", "nm_gated_tail_workspace_bytes"}
+             "nm_embed_bwd_workspace_bytes", "nm_gated_tail_workspace_bytes",
+             "nm_ce_distill_workspace_bytes"}
 
 IMPLS = {"A": 0, "B1": 1, "B1.5": 2, "B2": 3}
 LEV, ACC = 0, 1
@@ -187,3 +191,26 @@ def ce_call(lib, impl, x, W, targets, weight, gscale, *, rounding=LEV, store=BF1
         status = C.c_uint32(0)
         lib.nm_ce_device_status(ptr(ws), st, C.byref(status))
     return loss, lse
+
+
+def distill_call(lib, x, W, ids, teacher_logits, weight, gscale=None, *, tau=1.0, soft=1.0, hard=0.0, teacher_lse=None,
+                 targets=None, dx=None, acc_dx=False, dw=None, chunk=8192, loss_partial=None, ignore_index=-2 ** 31, ws=None,
+                 stream=None, check=True):
+    """Runs nm_ce_distill (forward only when neither dx nor dw is given). Returns (loss_tok, kl_tok, lse); dx / dw are
+    written in place. check: synchronise and read the device status word."""
+    import torch
+    T, D = x.shape
+    V, K = W.shape[0], ids.shape[1]
+    fwd = dx is None and dw is None
+    out = torch.empty(3, T, dtype=torch.float32, device=x.device)
+    if ws is None:
+        ws = Ws.get(lib.nm_ce_distill_workspace_bytes(T, D, V, K, chunk, int(fwd)), x.device)
+    st = None if stream is None else VP(stream)
+    lib.nm_ce_distill(int(teacher_logits.dtype == torch.bfloat16), ptr(x), ptr(W), ptr(ids), ptr(teacher_logits),
+                      ptr(teacher_lse), ptr(targets), ptr(weight), ptr(gscale), tau, soft, hard, ptr(out[0]), ptr(out[1]),
+                      ptr(out[2]), ptr(loss_partial), ptr(dx), int(acc_dx), ptr(dw), int(fwd), T, D, V, K, chunk, ignore_index,
+                      ptr(ws), ws.numel(), st)
+    if check and T > 0:
+        status = C.c_uint32(0)
+        lib.nm_ce_device_status(ptr(ws), st, C.byref(status))
+    return out[0], out[1], out[2]
