@@ -52,31 +52,43 @@ struct DistillRowsArgs {
   DistillRow* rowf; int32_t* pcol; float* pval;   // nullptr in a forward-only call; patches [rows, K + 1]
 };
 
-// 32 rows per CTA. First the tile partials are merged (lane = row, warp w takes the w-th eighth of the vocabulary's tiles,
-// warp 0 joins the eighths, all in ascending order), then each warp takes four rows, its lanes the listed entries.
-constexpr int kRowWarps = 8, kRowsPerCta = 32;
+// 32 rows per CTA. First the tile partials are merged (lane = row, warp w takes the w-th sixteenth of the vocabulary's tiles,
+// eight at a time so that their loads are in flight together; warp 0 joins the sixteenths, all in ascending order), then each
+// warp takes two rows, its lanes the listed entries. Bound by latency: a CTA waits for some ten dependent round trips.
+constexpr int kRowWarps = 16, kRowsPerCta = 32;
 __global__ void __launch_bounds__(32 * kRowWarps) k_distill_rows(const DistillRowsArgs p) {
   __shared__ float sm[kRowWarps][32], ss[kRowWarps][32], s1[kRowWarps][32];
   __shared__ float lse_t[32], lse_1[32];
-  __shared__ int32_t sid[kRowWarps][kMaxEntries];
-  __shared__ float sq[kRowWarps][kMaxEntries];
+  extern __shared__ int32_t entries[];   // per warp: ids [K], masses [K]
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const float inv_tau = __fdiv_rn(1.f, p.tau);
+  nm::ptx::release_next();
+  nm::ptx::after_previous();
   {
     const int r = blockIdx.x * kRowsPerCta + lane;
     const bool on = r < p.rows;
     const int i0 = int(int64_t(p.NT) * w / kRowWarps), i1 = int(int64_t(p.NT) * (w + 1) / kRowWarps);
     float m = -INFINITY, s = 0.f, o = 0.f;
     if (on) {
-#pragma unroll 8
-      for (int i = i0; i < i1; ++i) m = fmaxf(m, p.tmax[int64_t(i) * p.ldT + r]);
-      const float mm = isfinite(m) ? m : 0.f;
-#pragma unroll 4
-      for (int i = i0; i < i1; ++i) {
-        const int64_t at = int64_t(i) * p.ldT + r;
-        const float d = p.tmax[at] - mm;
-        s = fmaf(p.tsum[at], expf(d * inv_tau), s);
-        if (p.tsum1) o = fmaf(p.tsum1[at], expf(d), o);
+      for (int i = i0; i < i1; i += 8) {
+        float tm[8], ts[8], to[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int64_t at = int64_t(min(i + q, i1 - 1)) * p.ldT + r;
+          tm[q] = p.tmax[at], ts[q] = p.tsum[at], to[q] = p.tsum1 ? p.tsum1[at] : 0.f;
+        }
+        float nm = m;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) nm = fmaxf(nm, tm[q]);
+        const float base = isfinite(nm) ? nm : 0.f, back = isfinite(m) ? m - base : 0.f;   // no sums yet where m is not finite
+        s *= expf(back * inv_tau), o *= expf(back);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (i + q >= i1) break;
+          s = fmaf(ts[q], expf((tm[q] - base) * inv_tau), s);
+          if (p.tsum1) o = fmaf(to[q], expf(tm[q] - base), o);
+        }
+        m = nm;
       }
     }
     sm[w][lane] = m, ss[w][lane] = s, s1[w][lane] = o;
@@ -89,19 +101,19 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_distill_rows(const DistillRo
       float S = 0.f, O = 0.f;
 #pragma unroll
       for (int k = 0; k < kRowWarps; ++k) {
-        const float d = (isfinite(sm[k][lane]) ? sm[k][lane] : 0.f) - M;   // an empty eighth has sums of 0
+        const float d = (isfinite(sm[k][lane]) ? sm[k][lane] : 0.f) - M;   // an empty share has sums of 0
         S = fmaf(ss[k][lane], expf(d * inv_tau), S);
         O = fmaf(s1[k][lane], expf(d), O);
       }
       lse_t[lane] = logf(S) + M * inv_tau;
-      lse_1[lane] = p.tsum1 ? logf(O) + M : 0.f;
+      lse_1[lane] = p.tsum1 ? logf(O) + M : lse_t[lane];   // at temperature 1 one sum serves both
       p.lse[r] = lse_t[lane];
     }
     __syncthreads();
   }
   const float tau_log2e = kLog2e / p.tau;
-  int32_t* const id_s = sid[w];
-  float* const q_s = sq[w];
+  int32_t* const id_s = entries + w * 2 * p.K;
+  float* const q_s = reinterpret_cast<float*>(id_s + p.K);
   for (int j = 0; j < kRowsPerCta / kRowWarps; ++j) {
     const int local = w * (kRowsPerCta / kRowWarps) + j, r = blockIdx.x * kRowsPerCta + local;
     if (r >= p.rows) return;
@@ -201,6 +213,8 @@ __global__ void __launch_bounds__(256) k_distill_dots(const __nv_bfloat16* __res
                                                       const int32_t* __restrict__ ids, const float* __restrict__ weight,
                                                       int rows, int D, int V, int K, float* __restrict__ zk) {
   using namespace nm::ew;
+  nm::ptx::release_next();
+  nm::ptx::after_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int groups = (K + kDotEntries - 1) / kDotEntries;
   for (int64_t job = int64_t(blockIdx.x) * 8 + warp; job < int64_t(rows) * groups; job += int64_t(gridDim.x) * 8) {
@@ -250,6 +264,8 @@ __global__ void __launch_bounds__(kGradThreads) k_distill_grad(float* store, int
                                                                const int32_t* __restrict__ pcol,
                                                                const float* __restrict__ pval, int V, int patches,
                                                                float tau_log2e) {
+  nm::ptx::release_next();
+  nm::ptx::after_previous();
   const int r = blockIdx.y, c0 = blockIdx.x * kSegment, c1 = int(min(int64_t(c0) + kSegment, ldS));
   const DistillRow f = rowf[r];
   const bool dead = f.a_t == 0.f && f.a_1 == 0.f;
@@ -303,6 +319,8 @@ __global__ void __launch_bounds__(kGradThreads) k_distill_grad(float* store, int
 __global__ void __launch_bounds__(256) k_distill_dx_join(const float* __restrict__ part, int shares, int64_t n8,
                                                          const float* __restrict__ scale, __nv_bfloat16* dx, bool add) {
   using namespace nm::ew;
+  nm::ptx::release_next();
+  nm::ptx::after_previous();
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= n8) return;
   const float g = __ldg(scale);
@@ -393,7 +411,7 @@ void distill_head(const DistillHeadShape& s, const DistillHeadArgs& a, void* ws,
   NM_REQUIRE(device_arch() >= 100, "distillation: every kernel of this library is sm_100a code");
   const DistillRegions w = layout(s, ws);
   const int D = s.D, V = s.V, K = s.K;
-  const bool hard = a.hard_weight != 0.f;
+  const bool hard = a.hard_weight != 0.f, second_sum = hard && a.temperature != 1.f;
   const float tau_log2e = 1.4426950408889634f / a.temperature;
   const size_t teacher_size = dtype_size(a.teacher_dtype);
   NM_CUDA(cudaMemsetAsync(w.status, 0, sizeof(uint32_t), st));
@@ -404,7 +422,7 @@ void distill_head(const DistillHeadShape& s, const DistillHeadArgs& a, void* ws,
     const uint16_t* x = static_cast<const uint16_t*>(a.x) + r0 * D;
     const int32_t* ids = a.teacher_ids + r0 * K;
     DistillLogitsArgs la{x, a.w, hard ? a.targets + r0 : nullptr, n, D, V, a.temperature, grads ? w.store : nullptr, w.ldS,
-                         w.tmax, w.tsum, hard ? w.tsum1 : nullptr, n, w.zt, w.status};
+                         w.tmax, w.tsum, second_sum ? w.tsum1 : nullptr, n, w.zt, w.status};
     {
       ProfScope t(0, st);
       launch_distill_logits(la, st);
@@ -413,12 +431,12 @@ void distill_head(const DistillHeadShape& s, const DistillHeadArgs& a, void* ws,
     float* zk = s.forward_only ? w.zk : w.pval;
     if (!grads) {
       const int64_t jobs = int64_t(n) * ((K + kDotEntries - 1) / kDotEntries);
-      k_distill_dots<<<unsigned(std::min<int64_t>((jobs + 7) / 8, int64_t(sm_count()) * 64)), 256, 0, st>>>(
-          reinterpret_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a.w), ids, a.weight + r0, n, D, V, K, zk);
-      NM_CUDA(cudaGetLastError());
+      launch_after(k_distill_dots, dim3(unsigned(std::min<int64_t>((jobs + 7) / 8, int64_t(sm_count()) * 64))), 256, 0, st,
+                   reinterpret_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(a.w), ids, a.weight + r0, n, D, V,
+                   K, zk);
     }
     DistillRowsArgs ra{};
-    ra.tmax = w.tmax, ra.tsum = w.tsum, ra.tsum1 = hard ? w.tsum1 : nullptr, ra.ldT = n, ra.NT = stats_tiles(V);
+    ra.tmax = w.tmax, ra.tsum = w.tsum, ra.tsum1 = second_sum ? w.tsum1 : nullptr, ra.ldT = n, ra.NT = stats_tiles(V);
     ra.ids = ids, ra.logits = static_cast<const uint8_t*>(a.teacher_logits) + r0 * K * int64_t(teacher_size);
     ra.logits_bf16 = a.teacher_dtype == DType::bf16, ra.teacher_lse = a.teacher_lse ? a.teacher_lse + r0 : nullptr, ra.K = K;
     ra.targets = hard ? a.targets + r0 : nullptr, ra.weight = a.weight + r0, ra.zt = w.zt;
@@ -428,8 +446,10 @@ void distill_head(const DistillHeadShape& s, const DistillHeadArgs& a, void* ws,
     ra.rowf = grads ? w.rowf : nullptr, ra.pcol = w.pcol, ra.pval = w.pval;
     {
       ProfScope t(1, st);
-      k_distill_rows<<<(n + kRowsPerCta - 1) / kRowsPerCta, 32 * kRowWarps, 0, st>>>(ra);
-      NM_CUDA(cudaGetLastError());
+      const int entry_bytes = kRowWarps * 2 * K * 4;
+      if (entry_bytes > 32 * 1024)
+        NM_CUDA(cudaFuncSetAttribute(k_distill_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, entry_bytes));
+      launch_after(k_distill_rows, dim3(unsigned((n + kRowsPerCta - 1) / kRowsPerCta)), 32 * kRowWarps, unsigned(entry_bytes), st, ra);
     }
     if (a.loss_partial) {
       ProfScope t(5, st);
@@ -440,11 +460,10 @@ void distill_head(const DistillHeadShape& s, const DistillHeadArgs& a, void* ws,
       ProfScope t(2, st);
       for (int y0 = 0; y0 < n; y0 += 65535) {   // rows of one launch: the grid's second extent
         const int ny = std::min(n - y0, 65535);
-        k_distill_grad<<<dim3(unsigned((w.ldS + kSegment - 1) / kSegment), unsigned(ny)), kGradThreads, 0, st>>>(
-            w.store + int64_t(y0) * w.ldS, w.ldS, w.rowf + y0, w.pcol + int64_t(y0) * (K + 1), w.pval + int64_t(y0) * (K + 1), V,
-            K + 1, tau_log2e);
+        launch_after(k_distill_grad, dim3(unsigned((w.ldS + kSegment - 1) / kSegment), unsigned(ny)), kGradThreads, 0, st,
+                     w.store + int64_t(y0) * w.ldS, w.ldS, w.rowf + y0, w.pcol + int64_t(y0) * (K + 1),
+                     w.pval + int64_t(y0) * (K + 1), V, K + 1, tau_log2e);
       }
-      NM_CUDA(cudaGetLastError());
     }
     if (a.dw) {   // before dX, which may be written over x
       ProfScope t(3, st);
@@ -458,9 +477,8 @@ void distill_head(const DistillHeadShape& s, const DistillHeadArgs& a, void* ws,
                                             w.dxpart, shares, w.status}, st);
       if (shares > 1) {
         const int64_t n8 = int64_t(n) * D / 8;
-        k_distill_dx_join<<<unsigned((n8 + 255) / 256), 256, 0, st>>>(w.dxpart, shares, n8, a.grad_scale,
-                                                                     reinterpret_cast<__nv_bfloat16*>(dx), a.accumulate_dx);
-        NM_CUDA(cudaGetLastError());
+        launch_after(k_distill_dx_join, dim3(unsigned((n8 + 255) / 256)), 256, 0, st, w.dxpart, shares, n8, a.grad_scale,
+                     reinterpret_cast<__nv_bfloat16*>(dx), a.accumulate_dx);
       }
     }
   }

@@ -50,7 +50,7 @@ constexpr int smem_bytes(int epi, int ncta) {
 
 // ---------------------------------------------------------------------------------------------- the kernel
 // TWO (the distillation head's gradient contractions): A is the two-term gradient of ce_internal.hpp. dX (A K-major): K
-// block kb is the hi block kb, at column 128 kb; the tiles are dealt k_parts times, each time over its own k_part K blocks.
+// block kb is the hi block kb, at column 128 kb, or with p.k_terms = 2 the blocks alternate between the terms; the tiles are dealt k_parts times, each time over its own k_part K blocks.
 // dW (A MN-major): K blocks alternate between the terms of the same 64 rows; a CTA takes its tile k_parts times in a row,
 // k_part K blocks each, and its epilogue lets the additions of one part finish before it issues those of the next, so that
 // the order of additions is fixed.
@@ -107,9 +107,13 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if constexpr (EPI == kEpiDistill || TWO) {   // launched by launch_after's rule
+    release_next();
+    after_previous();
+  }
 
   const int num_tiles = TWO && !A_MN ? p.num_m * p.num_n * p.k_parts : p.num_m * p.num_n;
-  const int all_k_blocks = (p.K + BK - 1) / BK * (TWO && A_MN ? 2 : 1);
+  const int all_k_blocks = (p.K + BK - 1) / BK * (TWO ? p.k_terms : 1);
   const int parts = TWO && A_MN ? p.k_parts : 1;            // passes of a CTA over its tile
   // K blocks [kb0, kb1) of pass `part` over `tile`
   auto k_range = [&](int tile, int part, int& kb0, int& kb1) {
@@ -179,11 +183,11 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
           const uint32_t bar = NCTA == 2 ? mapa_shared(full_bar(stage), 0) : full_bar(stage);
           if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), NCTA * kStageBytes);
           const uint32_t a_dst = sA + stage * kABytes, b_dst = sB + stage * kBBytes;
-          const int k0 = (TWO && A_MN ? kb >> 1 : kb) * BK;
+          const int k0 = (TWO ? kb >> (p.k_terms - 1) : kb) * BK;
           if constexpr (TWO && A_MN) {
             tma_load_4d(a_dst, &tmA, bar, 0, k0, kb & 1, m0 >> 6);
           } else if constexpr (TWO) {
-            ld2(a_dst, &tmA, bar, 2 * k0, m0, keepA);
+            ld2(a_dst, &tmA, bar, p.k_terms == 2 ? kb * BK : 2 * k0, m0, keepA);
           } else if constexpr (A_MN) {
             if (p.a_3d) {
               ld3(a_dst, &tmA, bar, 0, k0, m0 >> 6, keepA);
@@ -493,6 +497,11 @@ void launch_n(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
   attr.val.clusterDim.x = NCTA; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = NCTA == 2 ? 1 : 0;
+  if ((EPI == kEpiDistill || TWO) && NCTA == 1) {
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
   NM_CUDA(cudaLaunchKernelEx(&cfg, kernel, ta, tb, tc, p));
 }
 template <int EPI, bool A_MN, bool B_MN>
@@ -602,7 +611,8 @@ void launch_distill_logits(const DistillLogitsArgs& a, cudaStream_t st) {
 // Of up to 16 shares the one with the fewest K blocks per SM is taken, a share counting 24 blocks more for its epilogue
 // and the reading of its sums; the sums take at most 32768 x D f32.
 int distill_dgrad_shares(int rows, int D, int V) {
-  const int64_t tiles = int64_t((rows + BM - 1) / BM) * ((D + BN - 1) / BN), kb = (V + BK - 1) / BK, sms = sm_count();
+  const int64_t tiles = int64_t((rows + BM - 1) / BM) * ((D + BN - 1) / BN), sms = sm_count();
+  const int64_t kb = (V + BK - 1) / BK * (rows <= kTwoTermDxRows ? 2 : 1);
   int best = 1;
   int64_t least = INT64_MAX;
   for (int s = 1; s <= 16 && int64_t(s) * rows <= 32768 && s <= kb; ++s) {
@@ -622,7 +632,8 @@ void launch_distill_dgrad(const DistillDgradArgs& a, cudaStream_t st) {
   p.status = a.status;
   p.scale = a.scale; p.dx_old = a.dx_old; p.dx_out = a.dx_out; p.acc_mode = a.dx_old ? a.acc_mode : 0; p.ldo = a.D;
   p.c = a.shares > 1 ? a.part : nullptr; p.ldc = a.D;
-  const int kb = (a.V + BK - 1) / BK;
+  p.k_terms = a.rows <= kTwoTermDxRows ? 2 : 1;
+  const int kb = (a.V + BK - 1) / BK * p.k_terms;
   p.k_part = (kb + a.shares - 1) / a.shares;
   p.k_parts = a.shares;
   NM_REQUIRE((p.k_parts - 1) * p.k_part < kb, "distillation: an empty share of the dX contraction");
@@ -638,8 +649,11 @@ void launch_distill_wgrad(const DistillWgradArgs& a, cudaStream_t st) {
   p.num_m = (a.V + BM - 1) / BM; p.num_n = (a.D + BN - 1) / BN; p.m_group = 1;
   p.status = a.status;
   p.scale = a.scale; p.dw = a.dw;
-  p.k_part = 2 * kDrainRows / BK;
-  p.k_parts = (a.rows + kDrainRows - 1) / kDrainRows;
+  // passes of equal length, in blocks of 64 rows of both terms
+  const int blocks = (a.rows + BK - 1) / BK, passes = (a.rows + kDrainRows - 1) / kDrainRows;
+  p.k_terms = 2;
+  p.k_part = 2 * ((blocks + passes - 1) / passes);
+  p.k_parts = (2 * blocks + p.k_part - 1) / p.k_part;
   const CUtensorMap ta = tmap_two_term_mn_a(a.n, a.rows, a.ldn);
   const CUtensorMap tb = tmap_mn_b(a.x, a.rows, a.D, a.D, p.b_3d, 1);
   const CUtensorMap tc = tmap_epilogue(a.dw, a.V, a.D, a.D, true);

@@ -87,6 +87,23 @@ GradPath grad_path_for(int D, int rows, bool plain_bf16);        // plain_bf16: 
 void set_tail_order(int order);
 int tail_order();
 
+// Launch in which the CTAs of `kernel` may be set up while the launch before it on the stream drains. The kernel executes
+// griddepcontrol.wait (ptx.cuh after_previous) before it touches anything that launch wrote or read.
+template <class Kernel, class... Args>
+void launch_after(Kernel kernel, dim3 grid, unsigned threads, unsigned smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NM_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 // Optional per-kernel-class timing for benches: when enabled, run() brackets every launch with a pair of CUDA events on
 // the call's stream (the events are created when profiling is enabled, never inside a call). Classes: 0 logits,
 // 1 finalize, 2 dlogits pass, 3 dW, 4 dX, 5 chunk loss.
@@ -170,10 +187,12 @@ void launch_distill_logits(const DistillLogitsArgs& a, cudaStream_t st);
 // The gradient n as two bf16 terms, hi + lo, in blocks of 64 columns: block b of hi at columns [128 b, 128 b + 64), of lo
 // behind it (row pitch ldn bf16 elements, a multiple of 128).
 //   dX: shares of the contraction over V are summed apart (part [shares, rows, D] f32, added up by the caller) when shares
-//       > 1; else the epilogue writes dx as DgradArgs does. Only hi is contracted: dx is stored in bf16.
-//   dW: both terms; the accumulator is drained into dw (f32) after every kDrainRows rows, because the tensor core adds to it
-//       with truncation (measured: the relative error of a contraction of length K grows as 1e-9 K).
-constexpr int kDrainRows = 1024;
+//       > 1; else the epilogue writes dx as DgradArgs does. Calls of more than kTwoTermDxRows rows contract hi alone (dx is
+//       stored in bf16, and the rounding of hi adds to it as one of its own does); up to that many rows, one M tile, the call
+//       reads W from HBM for longer than either form computes, and both terms are taken.
+//   dW: both terms; the accumulator is drained into dw (f32) after at most kDrainRows rows, because the tensor core adds to
+//       it with truncation (measured: the relative error of a contraction of length K grows as 1e-9 K).
+constexpr int kDrainRows = 1152, kTwoTermDxRows = 128;
 struct DistillDgradArgs {
   const void* n; int64_t ldn; const void* w;
   int rows, D, V;

@@ -52,7 +52,7 @@ struct GemmParams {
   float tau_log2e; float* tsum1;
   // contractions over a gradient held as two bf16 terms: K blocks per pass over the tile (segments drained one by one, dW)
   // and per share of a split contraction (dX), and the number of either
-  int k_part, k_parts;
+  int k_part, k_parts, k_terms;
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -147,29 +147,38 @@ struct DistillRowState {
 __device__ __forceinline__ void epi_distill_chunk(const GemmParams& p, const float* v, int col0, int tg, DistillRowState& st) {
   constexpr float kLog2e = 1.4426950408889634f;
   const int ncols = min(32, p.N - col0);
-  const bool whole = ncols == 32;
-  float cm = v[0];                          // the first column of a chunk exists
+  const float c = p.tau_log2e;
+  float m, a[4] = {}, b[4] = {};
+  if (ncols == 32) {                        // every chunk but the last of a ragged vocabulary: no column predicates
+    float t[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-  for (int j = 1; j < 32; ++j)
-    if (whole || j < ncols) cm = fmaxf(cm, v[j]);
-  const float m = fmaxf(st.m, cm), c = p.tau_log2e, neg = -m * c;
-  float a0 = 0.f, a1 = 0.f;
+    for (int j = 4; j < 32; ++j) t[j & 3] = fmaxf(t[j & 3], v[j]);
+    m = fmaxf(st.m, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+    const float neg = -m * c;
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
-    if (whole || j < ncols) a0 += ex2_approx(fmaf(v[j], c, neg));
-    if (whole || j + 1 < ncols) a1 += ex2_approx(fmaf(v[j + 1], c, neg));
-  }
-  st.s = st.s * ex2_approx(fmaf(st.m, c, neg)) + (a0 + a1);   // st.m == -inf on the first chunk: ex2(-inf) = 0
-  if (p.tsum1) {                            // uniform over the launch
-    const float neg1 = -m * kLog2e;
-    float b0 = 0.f, b1 = 0.f;
+    for (int j = 0; j < 32; ++j) a[j & 3] += ex2_approx(fmaf(v[j], c, neg));
+    if (p.tsum1) {                          // uniform over the launch
+      const float neg1 = -m * kLog2e;
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      if (whole || j < ncols) b0 += ex2_approx(fmaf(v[j], kLog2e, neg1));
-      if (whole || j + 1 < ncols) b1 += ex2_approx(fmaf(v[j + 1], kLog2e, neg1));
+      for (int j = 0; j < 32; ++j) b[j & 3] += ex2_approx(fmaf(v[j], kLog2e, neg1));
     }
-    st.s1 = st.s1 * ex2_approx(fmaf(st.m, kLog2e, neg1)) + (b0 + b1);
+  } else {
+    float t = v[0];                         // the first column of a chunk exists
+#pragma unroll
+    for (int j = 1; j < 32; ++j)
+      if (j < ncols) t = fmaxf(t, v[j]);
+    m = fmaxf(st.m, t);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (j < ncols) {
+        a[j & 3] += ex2_approx(fmaf(v[j], c, -m * c));
+        if (p.tsum1) b[j & 3] += ex2_approx(fmaf(v[j], kLog2e, -m * kLog2e));
+      }
+    }
   }
+  // st.m == -inf on the first chunk: ex2(-inf) = 0 and the sums are 0
+  st.s = st.s * ex2_approx(fmaf(st.m, c, -m * c)) + ((a[0] + a[1]) + (a[2] + a[3]));
+  if (p.tsum1) st.s1 = st.s1 * ex2_approx(fmaf(st.m, kLog2e, -m * kLog2e)) + ((b[0] + b[1]) + (b[2] + b[3]));
   st.m = m;
   if (tg >= col0 && tg < col0 + 32) {
     const int jt = tg - col0;

@@ -64,10 +64,8 @@ __device__ __forceinline__ void add32(float* p, const float* f) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]) : "memory");
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + 4), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]) : "memory");
 }
-// Between dependent launches of one call: the next kernel's CTAs may be set up while this one drains (`release`), and
-// wait for its completion before they touch what it wrote (`after_previous`).
-__device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+using nm::ptx::after_previous;
+using nm::ptx::release_next;
 
 // ------------------------------------------------------------------------------------------------ forward
 // G threads side by side on a row (eight elements each), kRows rows per group in flight: bound by HBM.
@@ -623,21 +621,10 @@ void require_arch(const char* who) {
   NM_REQUIRE(ce::device_arch() >= 100, std::string(who) + ": this library holds sm_100a code only");
 }
 
-// Launch whose CTAs may be set up while the launch before it drains; the kernel waits itself (after_previous).
 template <class Kernel, class Params>
 void launch_next(Kernel kernel, dim3 grid, int threads, int smem, const Params& p, cudaStream_t st) {
   if (smem > 48 * 1024) NM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(unsigned(threads));
-  cfg.dynamicSmemBytes = size_t(smem);
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  NM_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  ce::launch_after(kernel, grid, unsigned(threads), unsigned(smem), st, p);
 }
 
 template <int R>

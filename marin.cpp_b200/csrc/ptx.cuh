@@ -127,6 +127,11 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
   }
 }
 
+// Between dependent launches (programmatic stream serialisation): the next kernel's CTAs may be set up while this one
+// drains (release_next), and wait for its completion before they touch what it wrote (after_previous).
+__device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------------------------------------------------------------------------ TMA
 // 2-D tiled load global -> shared, completion counted in bytes on an mbarrier of this CTA. c0 is the innermost
 // coordinate (elements); c0 * element size must be a multiple of 16 bytes.

@@ -6,7 +6,7 @@ roundings of their exponents (a few u times the size of the numbers in them; 64 
 exponentials of 2 ulp, the merges and the sums). So a probability is off by at most rho = 2 Z / tau + that, relative, a
 divergence by (1 + mass) times rho, an element of n by rho times the sizes of its parts. dW takes n as two bf16 terms (each
 half a step: 2^-8 * 2^-8 < 2^-15 would be the bound of the second term's rounding of a first remainder of 2^-8: 2^-16 of n) and adds
-at most 1024 rows x 2 terms before it drains: 1024 / 8 steps of 2 u. dX takes the first term alone (2^-8 of n), adds V / 16 steps
+at most 1152 rows x 2 terms before it drains: 1152 / 8 steps of 2 u. dX takes the first term alone (2^-8 of n; both in short calls), adds up to V / 8 steps
 of 2 u (all shares together), and is stored with half a step of bf16."""
 import ctypes
 
@@ -88,14 +88,14 @@ def _check(c, soft, hard, out, dx=None, dw=None, ignore=BIG_NEG, dx0=None, dw0=N
     n, dn = f["n"].abs(), f["dn"]
     if dw is not None:
         want, size = g * (f["n"].T @ c["x"].double()), g * (n.T @ c["x"].double().abs())
-        tol = g * (dn.T @ c["x"].double().abs()) + (2.0 ** -16 + (1024 / 8 + c["x"].shape[0] / 1024 + 4) * 2 * U) * size
+        tol = g * (dn.T @ c["x"].double().abs()) + (2.0 ** -16 + (1152 / 8 + c["x"].shape[0] / 1024 + 4) * 2 * U) * size
         if dw0 is not None:
             want = want + dw0.double()
             tol = tol + (c["x"].shape[0] / 1024 + 2) * U * (dw0.double().abs() + size)
         _close("dw", dw, want, tol + 1e-30)
     if dx is not None:
         want, size = g * (f["n"] @ c["w"].double()), g * (n @ c["w"].double().abs())
-        tol = g * (dn @ c["w"].double().abs()) + (2.0 ** -8 + (c["w"].shape[0] / 16 + 40) * 2 * U) * size
+        tol = g * (dn @ c["w"].double().abs()) + (2.0 ** -8 + (c["w"].shape[0] / 8 + 40) * 2 * U) * size
         if dx0 is not None:
             want = want + dx0.double()
         _close("dx", dx, want, tol + 2.0 ** -8 * (want.abs() + tol) + 1e-30)
