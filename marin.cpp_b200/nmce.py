@@ -135,16 +135,19 @@ class Lib:
             if name not in NO_STATUS and r != 0:
                 raise NmError(name, r, self.dll.nm_last_error().decode())
             return r
+        self.__dict__[name] = call      # the next use finds it without coming here
         return call
 
 
 def ptr(t):
-    """Device (or host) pointer of a torch tensor / numpy array, None for None."""
+    """Device (or host) address of a torch tensor / numpy array as a plain integer, None for None (what a c_void_p argument
+    takes; a c_void_p object made for every argument costs a short call several microseconds)."""
     if t is None:
         return None
-    if hasattr(t, "data_ptr"):
-        return VP(t.data_ptr())
-    return VP(t.ctypes.data)
+    try:
+        return t.data_ptr()
+    except AttributeError:
+        return t.ctypes.data
 
 
 class Ws:
