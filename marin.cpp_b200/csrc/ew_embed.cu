@@ -318,9 +318,10 @@ __global__ void __launch_bounds__(kSortThreads, 1) k_embed_sort(const SortParams
 // runs are never cut, no window has more than 2.5 win rows to read, and a cut costs 8 bytes of f32 traffic per column
 // for at least win / 2 rows read.
 constexpr int kNoKey = INT_MAX;
-// Measured for 131072 tokens of width 2048 (ids falling as 1 / rank): windows of 64 rows 297 us for the whole call, of 32
-// rows 305 us (twice the cut pieces). Short sections take 32: there are then enough windows to fill the SMs.
-inline int window_for(int64_t n) { return n > 32768 ? 64 : 32; }
+// Measured for the whole call: 131072 tokens of width 2048 (ids falling as 1 / rank), windows of 64 rows 297 us, of 32 rows
+// 305 us (twice the cut pieces); 2125 tokens of width 768 in f32, windows of 32 rows 26 us, of 16 rows 20.5 us (a short
+// section waits for the longest window).
+inline int window_for(int64_t n) { return n > 32768 ? 64 : n > 2560 ? 32 : 16; }
 
 struct ReduceParams {
   const void* dy;
