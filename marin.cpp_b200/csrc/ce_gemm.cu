@@ -47,12 +47,17 @@ __host__ __device__ constexpr int epi_stage_bytes(int epi) {
 constexpr int smem_bytes(int epi, int ncta) {
   return num_stages(ncta) * stage_bytes(ncta) + epi_stage_bytes(epi) + 1024 /*alignment slack*/ + 256 /*barriers*/;
 }
+// dW over a two-term gradient: a stage holds both terms' A tiles and the B tile that they share (64 KiB, three stages)
+constexpr int kTwoTermStages = 3, kTwoTermStageBytes = 2 * kABytes + b_bytes(1);
+constexpr int two_term_smem_bytes() {
+  return kTwoTermStages * kTwoTermStageBytes + epi_stage_bytes(kEpiDw) + 1024 + 256;
+}
 
 // ---------------------------------------------------------------------------------------------- the kernel
 // TWO (the distillation head's gradient contractions): A is the two-term gradient of ce_internal.hpp. dX (A K-major): K
 // block kb is the hi block kb, at column 128 kb, or with p.k_terms = 2 the blocks alternate between the terms; the tiles are dealt k_parts times, each time over its own k_part K blocks.
-// dW (A MN-major): K blocks alternate between the terms of the same 64 rows; a CTA takes its tile k_parts times in a row,
-// k_part K blocks each, and its epilogue lets the additions of one part finish before it issues those of the next, so that
+// dW (A MN-major): a stage holds both terms of 64 rows and the 64 rows of x that they share; a CTA takes its tile k_parts
+// times in a row, k_part K blocks (counted per term) each, and its epilogue lets the additions of one part finish before it issues those of the next, so that
 // the order of additions is fixed.
 template <int EPI, bool A_MN, bool B_MN, int NCTA, bool TWO = false>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -62,10 +67,12 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;            // SWIZZLE_128B tiles need 1024-byte alignment
   uint8_t* smem = smem_raw + (base - raw);
-  constexpr int kStages = num_stages(NCTA), kBBytes = b_bytes(NCTA), kStageBytes = stage_bytes(NCTA);
+  constexpr int kTerms = TWO && A_MN ? 2 : 1;              // A tiles per stage
+  constexpr int kStages = kTerms == 2 ? kTwoTermStages : num_stages(NCTA), kBBytes = b_bytes(NCTA);
+  constexpr int kAStage = kTerms * kABytes, kStageBytes = kAStage + kBBytes;
   constexpr int BMT = BM * NCTA;                           // accumulator rows of one tile (all CTAs of the pair)
   constexpr int BNC = BN / NCTA;                           // B columns this CTA stages
-  const uint32_t sA = base, sB = base + kStages * kABytes;
+  const uint32_t sA = base, sB = base + kStages * kAStage;
   const uint32_t sEpi = base + kStages * kStageBytes;      // epilogue staging tiles (1024-byte aligned)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes + epi_stage_bytes(EPI));
   const uint32_t bar0 = sEpi + epi_stage_bytes(EPI);
@@ -178,14 +185,15 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         int kb0, kb1;
         k_range(tile, 0, kb0, kb1);
         if constexpr (TWO && A_MN) kb1 = all_k_blocks;       // the passes follow one another
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = kb0; kb < kb1; kb += kTerms) {
           if (!mbar_wait<true>(empty_bar(stage), phase ^ 1u, abort_flag, p.status, kErrProducerWait)) { ok = false; break; }
           const uint32_t bar = NCTA == 2 ? mapa_shared(full_bar(stage), 0) : full_bar(stage);
           if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), NCTA * kStageBytes);
-          const uint32_t a_dst = sA + stage * kABytes, b_dst = sB + stage * kBBytes;
+          const uint32_t a_dst = sA + stage * kAStage, b_dst = sB + stage * kBBytes;
           const int k0 = (TWO ? kb >> (p.k_terms - 1) : kb) * BK;
           if constexpr (TWO && A_MN) {
-            tma_load_4d(a_dst, &tmA, bar, 0, k0, kb & 1, m0 >> 6);
+            tma_load_4d(a_dst, &tmA, bar, 0, k0, 0, m0 >> 6);
+            tma_load_4d(a_dst + kABytes, &tmA, bar, 0, k0, 1, m0 >> 6);
           } else if constexpr (TWO) {
             ld2(a_dst, &tmA, bar, p.k_terms == 2 ? kb * BK : 2 * k0, m0, keepA);
           } else if constexpr (A_MN) {
@@ -227,19 +235,21 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         if (!mbar_wait(tempty_bar(b), ((it >> 1) & 1u) ^ 1u, abort_flag, p.status, kErrTmemFreeWait)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + uint32_t(b * BN);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = kb0; kb < kb1; kb += kTerms) {
           if (!mbar_wait(full_bar(stage), phase, abort_flag, p.status, kErrMmaWait)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_src = sA + stage * kABytes, b_src = sB + stage * kBBytes;
+          const uint32_t a_first = sA + stage * kAStage, b_src = sB + stage * kBBytes;
 #pragma unroll
-          for (int k = 0; k < BK / UK; ++k) {
+          for (int kk = 0; kk < kTerms * (BK / UK); ++kk) {
+            const int k = kk % (BK / UK);
+            const uint32_t a_src = a_first + (kk / (BK / UK)) * kABytes;
             // K-major: 16 bf16 = 32 bytes further along the 128-byte row; MN-major: 16 k-rows = 2048 bytes further
             const uint64_t ad = A_MN ? smem_desc_sw128(a_src + k * (UK * 128), kBoxBytesMN, 1024)
                                      : smem_desc_sw128(a_src + k * (UK * 2), 16, 1024);
             const uint64_t bd = B_MN ? smem_desc_sw128(b_src + k * (UK * 128), kBoxBytesMN, 1024)
                                      : smem_desc_sw128(b_src + k * (UK * 2), 16, 1024);
-            if constexpr (NCTA == 2) umma_pair_bf16(d_tmem, ad, bd, idesc, kb != kb0 || k != 0);
-            else umma_bf16(d_tmem, ad, bd, idesc, kb != kb0 || k != 0);
+            if constexpr (NCTA == 2) umma_pair_bf16(d_tmem, ad, bd, idesc, kb != kb0 || kk != 0);
+            else umma_bf16(d_tmem, ad, bd, idesc, kb != kb0 || kk != 0);
           }
           // the stage is free again once these UMMAs have read it (pair mode: in both CTAs)
           if constexpr (NCTA == 2) umma_pair_commit(empty_bar(stage), 3);
@@ -481,7 +491,7 @@ template <int EPI, bool A_MN, bool B_MN, int NCTA, bool TWO = false>
 void launch_n(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const GemmParams& p,
               cudaStream_t st, int sm_reserve) {
   auto kernel = k_ce_umma<EPI, A_MN, B_MN, NCTA, TWO>;
-  constexpr int kSmem = smem_bytes(EPI, NCTA);
+  constexpr int kSmem = TWO && A_MN ? two_term_smem_bytes() : smem_bytes(EPI, NCTA);
   static_assert(kSmem <= 232448, "dynamic shared memory beyond the 227 KiB a CTA may use");
   NM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   const int tiles = p.num_m * p.num_n * (TWO && !A_MN ? p.k_parts : 1);
