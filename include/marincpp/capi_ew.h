@@ -37,7 +37,8 @@ int nm_norm_bwd_device_status(void* stream, uint32_t* status_host);
 int nm_norm_bwd_test_timeout(int64_t limit_cycles, void* stream);
 
 /* ---- embedding (the reference's trunk has its own, src/kernels/elementwise/embed.cu; names and workspace here are this
- * library's). dtype: storage of table / out / dy, 1 = bf16, 0 = f32. D % 8 == 0, rows contiguous and 16-byte aligned.
+ * library's). dtype: storage of table / out / dy, 1 = bf16, 0 = f32. D % 8 == 0, D <= 65536, rows contiguous and
+ * 16-byte aligned.
  * forward:  out[t, :] = round(scale * table[tokens[t], :]), one rounding; a token outside [0, V) gives a row of zeros. */
 int nm_embed_fwd(int dtype, const void* table, const int32_t* tokens, void* out, float scale, int64_t T, int D, int V,
                  void* stream);

@@ -52,24 +52,23 @@ struct DistillRowsArgs {
   DistillRow* rowf; int32_t* pcol; float* pval;   // nullptr in a forward-only call; patches [rows, K + 1]
 };
 
-// 32 rows per CTA. First the tile partials are merged (lane = row, warp w takes the w-th sixteenth of the vocabulary's tiles,
-// eight at a time so that their loads are in flight together; warp 0 joins the sixteenths, all in ascending order), then each
-// warp takes two rows, its lanes the listed entries. Bound by latency: a CTA waits for some ten dependent round trips.
-constexpr int kRowWarps = 16, kRowsPerCta = 32;
-__global__ void __launch_bounds__(32 * kRowWarps) k_distill_rows(const DistillRowsArgs p) {
-  __shared__ float sm[kRowWarps][32], ss[kRowWarps][32], s1[kRowWarps][32];
-  __shared__ float lse_t[32], lse_1[32];
+// Eight rows per CTA. First the tile partials are merged: the vocabulary's tiles are cut into 32 strips, lane = (row, one of
+// four strips) of a warp, eight tiles at a time so that their loads are in flight together, in ascending order; then warp w
+// joins the strips of row w (a butterfly: the same order always) and stays with that row, its lanes the listed entries. Bound
+// by latency: a CTA waits for some ten dependent round trips. (With 32 rows per CTA 25 us instead of 12 us for 2125 rows.)
+constexpr int kRowsPerCta = 8, kStrips = 32;
+__global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const DistillRowsArgs p) {
+  __shared__ float sm[kStrips][kRowsPerCta], ss[kStrips][kRowsPerCta], s1[kStrips][kRowsPerCta];
   extern __shared__ int32_t entries[];   // per warp: ids [K], masses [K]
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const float inv_tau = __fdiv_rn(1.f, p.tau);
   nm::ptx::release_next();
   nm::ptx::after_previous();
   {
-    const int r = blockIdx.x * kRowsPerCta + lane;
-    const bool on = r < p.rows;
-    const int i0 = int(int64_t(p.NT) * w / kRowWarps), i1 = int(int64_t(p.NT) * (w + 1) / kRowWarps);
+    const int local = lane & 7, strip = w * 4 + (lane >> 3), r = blockIdx.x * kRowsPerCta + local;
+    const int i0 = int(int64_t(p.NT) * strip / kStrips), i1 = int(int64_t(p.NT) * (strip + 1) / kStrips);
     float m = -INFINITY, s = 0.f, o = 0.f;
-    if (on) {
+    if (r < p.rows) {
       for (int i = i0; i < i1; i += 8) {
         float tm[8], ts[8], to[8];
 #pragma unroll
@@ -91,118 +90,112 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_distill_rows(const DistillRo
         m = nm;
       }
     }
-    sm[w][lane] = m, ss[w][lane] = s, s1[w][lane] = o;
+    sm[strip][local] = m, ss[strip][local] = s, s1[strip][local] = o;
     __syncthreads();
-    if (w == 0 && on) {
-      float M = -INFINITY;
+  }
+  const int r = blockIdx.x * kRowsPerCta + w;
+  if (r >= p.rows) return;
+  float lt, l1;
+  {
+    float m = sm[lane][w], M = m;
 #pragma unroll
-      for (int k = 0; k < kRowWarps; ++k) M = fmaxf(M, sm[k][lane]);
-      if (!isfinite(M)) M = 0.f;
-      float S = 0.f, O = 0.f;
-#pragma unroll
-      for (int k = 0; k < kRowWarps; ++k) {
-        const float d = (isfinite(sm[k][lane]) ? sm[k][lane] : 0.f) - M;   // an empty share has sums of 0
-        S = fmaf(ss[k][lane], expf(d * inv_tau), S);
-        O = fmaf(s1[k][lane], expf(d), O);
-      }
-      lse_t[lane] = logf(S) + M * inv_tau;
-      lse_1[lane] = p.tsum1 ? logf(O) + M : lse_t[lane];   // at temperature 1 one sum serves both
-      p.lse[r] = lse_t[lane];
-    }
-    __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (!isfinite(M)) M = 0.f;
+    const float d = isfinite(m) ? m - M : 0.f;   // an empty strip has sums of 0
+    const float S = warp_sum(ss[lane][w] * expf(d * inv_tau));
+    lt = logf(S) + M * inv_tau;
+    l1 = lt;                                     // at temperature 1 one sum serves both
+    if (p.tsum1) l1 = logf(warp_sum(s1[lane][w] * expf(d))) + M;
+    if (lane == 0) p.lse[r] = lt;
   }
   const float tau_log2e = kLog2e / p.tau;
   int32_t* const id_s = entries + w * 2 * p.K;
   float* const q_s = reinterpret_cast<float*>(id_s + p.K);
-  for (int j = 0; j < kRowsPerCta / kRowWarps; ++j) {
-    const int local = w * (kRowsPerCta / kRowWarps) + j, r = blockIdx.x * kRowsPerCta + local;
-    if (r >= p.rows) return;
-    const float wt = p.weight[r], lt = lse_t[local], l1 = lse_1[local];
-    const bool live = wt != 0.f;
-    const int tg = p.targets ? p.targets[r] : -1;
-    const bool labelled = live && p.hard != 0.f && tg >= 0 && tg < p.V && tg != p.ignore_index;
-    const int64_t row_k = int64_t(r) * p.K;
-    // the listed entries of this row: id (or -1) and t / tau
-    auto scaled = [&](int k) {
-      const float t = p.logits_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[row_k + k])
-                                    : static_cast<const float*>(p.logits)[row_k + k];
-      return __fdiv_rn(t, p.tau);
-    };
-    __syncwarp();
-    float top = -INFINITY;
-    for (int k = lane; k < p.K; k += 32) {
-      const int32_t id = p.ids[row_k + k];
-      const bool in = live && id >= 0 && id < p.V;
-      id_s[k] = in ? id : -1;
-      if (in && !p.teacher_lse) top = fmaxf(top, scaled(k));
-    }
-    float norm = 0.f;
-    bool any = false;
-    if (p.teacher_lse) {
-      norm = p.teacher_lse[r];
-    } else {
+  const float wt = p.weight[r];
+  const bool live = wt != 0.f;
+  const int tg = p.targets ? p.targets[r] : -1;
+  const bool labelled = live && p.hard != 0.f && tg >= 0 && tg < p.V && tg != p.ignore_index;
+  const int64_t row_k = int64_t(r) * p.K;
+  // the listed entries of this row: id (or -1) and t / tau
+  auto scaled = [&](int k) {
+    const float t = p.logits_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[row_k + k])
+                                  : static_cast<const float*>(p.logits)[row_k + k];
+    return __fdiv_rn(t, p.tau);
+  };
+  __syncwarp();
+  float top = -INFINITY;
+  for (int k = lane; k < p.K; k += 32) {
+    const int32_t id = p.ids[row_k + k];
+    const bool in = live && id >= 0 && id < p.V;
+    id_s[k] = in ? id : -1;
+    if (in && !p.teacher_lse) top = fmaxf(top, scaled(k));
+  }
+  float norm = 0.f;
+  bool any = false;
+  if (p.teacher_lse) {
+    norm = p.teacher_lse[r];
+  } else {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      any = top != -INFINITY;
-      float s = 0.f;
-      for (int k = lane; k < p.K; k += 32)
-        if (id_s[k] >= 0 && any) s += expf(scaled(k) - top);
-      s = warp_sum(s);
-      norm = any ? top + logf(s) : INFINITY;      // nothing listed: every mass is 0
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    any = top != -INFINITY;
+    float s = 0.f;
+    for (int k = lane; k < p.K; k += 32)
+      if (id_s[k] >= 0 && any) s += expf(scaled(k) - top);
+    s = warp_sum(s);
+    norm = any ? top + logf(s) : INFINITY;      // nothing listed: every mass is 0
+  }
+  float kl = 0.f, mass = 0.f;
+  for (int k = lane; k < p.K; k += 32) {
+    const int32_t id = id_s[k];
+    float q = 0.f;
+    if (id >= 0) {
+      const float lq = scaled(k) - norm;
+      q = expf(lq);
+      const float z = p.store ? p.store[int64_t(r) * p.ldS + id] : p.zk[row_k + k];
+      if (q != 0.f) kl = fmaf(q, lq - fmaf(z, inv_tau, -lt), kl);
     }
-    float kl = 0.f, mass = 0.f;
-    for (int k = lane; k < p.K; k += 32) {
-      const int32_t id = id_s[k];
+    q_s[k] = q;
+    mass += q;
+  }
+  kl = warp_sum(kl);
+  mass = warp_sum(mass);
+  if (!p.teacher_lse) mass = any ? 1.f : mass;   // by definition (a NaN among the logits shows in kl)
+  if (lane == 0) {
+    float loss = 0.f;
+    if (live) {
+      loss = p.soft * p.tau * p.tau * kl;
+      if (labelled) loss = fmaf(p.hard, l1 - p.zt[r], loss);
+    }
+    p.loss[r] = loss;
+    if (p.kl) p.kl[r] = live ? kl : 0.f;
+  }
+  if (p.rowf == nullptr) return;
+  DistillRow f{0.f, 0.f, 0.f, 0.f};
+  const float unit = live ? wt * p.soft * p.tau : 0.f;   // gradient of one unit of teacher mass
+  const float hit = labelled ? wt * p.hard : 0.f;
+  if (live) f = DistillRow{-lt * kLog2e, unit * mass, -l1 * kLog2e, hit};
+  if (lane == 0) p.rowf[r] = f;
+  __syncwarp();
+  // the elements of n that are not dense alone, whole: every listed id, and the target where it is not listed
+  const int64_t row_p = int64_t(r) * (p.K + 1);
+  bool listed = false;
+  for (int k = lane; k < p.K; k += 32) {
+    const int32_t id = id_s[k];
+    float v = 0.f;
+    if (id >= 0) {
       float q = 0.f;
-      if (id >= 0) {
-        const float lq = scaled(k) - norm;
-        q = expf(lq);
-        const float z = p.store ? p.store[int64_t(r) * p.ldS + id] : p.zk[row_k + k];
-        if (q != 0.f) kl = fmaf(q, lq - fmaf(z, inv_tau, -lt), kl);
-      }
-      q_s[k] = q;
-      mass += q;
+      for (int o = 0; o < p.K; ++o) q += id_s[o] == id ? q_s[o] : 0.f;   // the same id twice: both write this sum
+      v = fmaf(-unit, q, dense_part(p.store[int64_t(r) * p.ldS + id], f, tau_log2e));
+      if (labelled && id == tg) v -= hit, listed = true;
     }
-    kl = warp_sum(kl);
-    mass = warp_sum(mass);
-    if (!p.teacher_lse) mass = any ? 1.f : mass;   // by definition (a NaN among the logits shows in kl)
-    if (lane == 0) {
-      float loss = 0.f;
-      if (live) {
-        loss = p.soft * p.tau * p.tau * kl;
-        if (labelled) loss = fmaf(p.hard, l1 - p.zt[r], loss);
-      }
-      p.loss[r] = loss;
-      if (p.kl) p.kl[r] = live ? kl : 0.f;
-    }
-    if (p.rowf == nullptr) continue;
-    DistillRow f{0.f, 0.f, 0.f, 0.f};
-    const float unit = live ? wt * p.soft * p.tau : 0.f;   // gradient of one unit of teacher mass
-    const float hit = labelled ? wt * p.hard : 0.f;
-    if (live) f = DistillRow{-lt * kLog2e, unit * mass, -l1 * kLog2e, hit};
-    if (lane == 0) p.rowf[r] = f;
-    __syncwarp();
-    // the elements of n that are not dense alone, whole: every listed id, and the target where it is not listed
-    const int64_t row_p = int64_t(r) * (p.K + 1);
-    bool listed = false;
-    for (int k = lane; k < p.K; k += 32) {
-      const int32_t id = id_s[k];
-      float v = 0.f;
-      if (id >= 0) {
-        float q = 0.f;
-        for (int o = 0; o < p.K; ++o) q += id_s[o] == id ? q_s[o] : 0.f;   // the same id twice: both write this sum
-        v = fmaf(-unit, q, dense_part(p.store[int64_t(r) * p.ldS + id], f, tau_log2e));
-        if (labelled && id == tg) v -= hit, listed = true;
-      }
-      p.pcol[row_p + k] = id;
-      p.pval[row_p + k] = v;
-    }
-    listed = __any_sync(0xffffffffu, listed);
-    if (lane == 0) {
-      const bool own = labelled && !listed;
-      p.pcol[row_p + p.K] = own ? tg : -1;
-      p.pval[row_p + p.K] = own ? dense_part(p.zt[r], f, tau_log2e) - hit : 0.f;
-    }
+    p.pcol[row_p + k] = id;
+    p.pval[row_p + k] = v;
+  }
+  listed = __any_sync(0xffffffffu, listed);
+  if (lane == 0) {
+    const bool own = labelled && !listed;
+    p.pcol[row_p + p.K] = own ? tg : -1;
+    p.pval[row_p + p.K] = own ? dense_part(p.zt[r], f, tau_log2e) - hit : 0.f;
   }
 }
 
@@ -446,10 +439,8 @@ void distill_head(const DistillHeadShape& s, const DistillHeadArgs& a, void* ws,
     ra.rowf = grads ? w.rowf : nullptr, ra.pcol = w.pcol, ra.pval = w.pval;
     {
       ProfScope t(1, st);
-      const int entry_bytes = kRowWarps * 2 * K * 4;
-      if (entry_bytes > 32 * 1024)
-        NM_CUDA(cudaFuncSetAttribute(k_distill_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, entry_bytes));
-      launch_after(k_distill_rows, dim3(unsigned((n + kRowsPerCta - 1) / kRowsPerCta)), 32 * kRowWarps, unsigned(entry_bytes), st, ra);
+      const int entry_bytes = kRowsPerCta * 2 * K * 4;
+      launch_after(k_distill_rows, dim3(unsigned((n + kRowsPerCta - 1) / kRowsPerCta)), 32 * kRowsPerCta, unsigned(entry_bytes), st, ra);
     }
     if (a.loss_partial) {
       ProfScope t(5, st);

@@ -34,6 +34,9 @@ struct Eight<true> {
   __device__ __forceinline__ static void store(void* p, int64_t at, const float* f) {
     *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at) = pack8(f);
   }
+  __device__ __forceinline__ static void stream(void* p, int64_t at, const float* f) {   // not read again soon
+    __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at), pack8(f));
+  }
 };
 template <>
 struct Eight<false> {
@@ -49,6 +52,11 @@ struct Eight<false> {
     float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
     d[0] = make_float4(f[0], f[1], f[2], f[3]);
     d[1] = make_float4(f[4], f[5], f[6], f[7]);
+  }
+  __device__ __forceinline__ static void stream(void* p, int64_t at, const float* f) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+    __stcs(d, make_float4(f[0], f[1], f[2], f[3]));
+    __stcs(d + 1, make_float4(f[4], f[5], f[6], f[7]));
   }
 };
 
@@ -68,31 +76,49 @@ using nm::ptx::after_previous;
 using nm::ptx::release_next;
 
 // ------------------------------------------------------------------------------------------------ forward
-// G threads side by side on a row (eight elements each), kRows rows per group in flight: bound by HBM.
-constexpr int kFwdRows = 4;
+// G threads side by side on a row (eight elements each); a row group takes `batches` times kFwdRows consecutive rows, the
+// loads of a batch in flight while the one before it is stored. Bound by HBM: the output is written once, past the L2 (the
+// frequent rows of the table are read from there again and again).
+constexpr int kFwdRows = 4, kFwdMaxBatches = 4;
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads) k_embed_fwd(const void* __restrict__ table, const int32_t* __restrict__ tokens,
-                                                        void* __restrict__ out, float scale, int64_t T, int D, int V, int G) {
-  const int groups = kThreads / G, pieces = D / 8;
-  const int64_t row0 = (int64_t(blockIdx.x) * groups + threadIdx.x / G) * kFwdRows;
-  int32_t tok[kFwdRows];
+                                                        void* __restrict__ out, float scale, int64_t T, int D, int V, int G,
+                                                        int batches) {
+  __shared__ int32_t tok_s[kThreads / 32 * kFwdRows * kFwdMaxBatches];
+  const int groups = kThreads / G, pieces = D / 8, g = threadIdx.x / G, tg = threadIdx.x % G;
+  const int rows = kFwdRows * batches;                       // per group
+  const int64_t row0 = (int64_t(blockIdx.x) * groups + g) * rows;
+  int32_t* const tok = tok_s + g * rows;
+  for (int u = tg; u < rows; u += G) {
+    const int32_t t = row0 + u < T ? __ldg(tokens + row0 + u) : -1;
+    tok[u] = uint32_t(t) < uint32_t(V) ? t : -1;
+  }
+  __syncthreads();
+  for (int pc = tg; pc < pieces; pc += G) {
+    Eight<BF16> e[kFwdRows], next[kFwdRows];
+    auto fetch = [&](Eight<BF16>(&to)[kFwdRows], int at) {
 #pragma unroll
-  for (int u = 0; u < kFwdRows; ++u) tok[u] = row0 + u < T ? __ldg(tokens + row0 + u) : -1;
-  for (int pc = threadIdx.x % G; pc < pieces; pc += G) {
-    Eight<BF16> e[kFwdRows];
-#pragma unroll
-    for (int u = 0; u < kFwdRows; ++u)
-      if (uint32_t(tok[u]) < uint32_t(V)) e[u].load(table, int64_t(tok[u]) * D + pc * 8);
-#pragma unroll
-    for (int u = 0; u < kFwdRows; ++u) {
-      if (row0 + u >= T) break;
-      float f[8] = {};
-      if (uint32_t(tok[u]) < uint32_t(V)) {
-        e[u].get(f);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] *= scale;
+      for (int u = 0; u < kFwdRows; ++u) {
+        const int32_t t = tok[at + u];
+        if (t >= 0) to[u].load(table, int64_t(t) * D + pc * 8);
       }
-      Eight<BF16>::store(out, (row0 + u) * D + pc * 8, f);
+    };
+    fetch(e, 0);
+    for (int at = 0; at < rows; at += kFwdRows) {
+      if (at + kFwdRows < rows) fetch(next, at + kFwdRows);
+#pragma unroll
+      for (int u = 0; u < kFwdRows; ++u) {
+        if (row0 + at + u >= T) break;
+        float f[8] = {};
+        if (tok[at + u] >= 0) {
+          e[u].get(f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f[k] *= scale;
+        }
+        Eight<BF16>::stream(out, (row0 + at + u) * D + pc * 8, f);
+      }
+#pragma unroll
+      for (int u = 0; u < kFwdRows; ++u) e[u] = next[u];
     }
   }
 }
@@ -616,6 +642,7 @@ void require_shape(int64_t T, int D, int V, const char* who) {
   const std::string w(who);
   NM_REQUIRE(T >= 0, w + ": the row count T cannot be negative");
   NM_REQUIRE(D > 0 && D % 8 == 0, w + ": D must be a positive multiple of 8 (rows are moved in 16-byte pieces)");
+  NM_REQUIRE(D <= 65536, w + ": D <= 65536");   // row offsets of a section are 32-bit counts of 16-byte pieces
   NM_REQUIRE(V > 0, w + ": the vocabulary size V must be positive");
 }
 void require_arch(const char* who) {
@@ -657,10 +684,13 @@ void embed_fwd(bool bf16, const void* table, const int32_t* tokens, void* out, f
   NM_REQUIRE(reinterpret_cast<uintptr_t>(tokens) % 4 == 0, "embed_fwd: tokens must be 4-byte aligned");
   require_arch("embed_fwd");
   const int G = threads_per_row(D / 8);
-  const int64_t per_cta = int64_t(kThreads / G) * kFwdRows, grid = (T + per_cta - 1) / per_cta;
+  // one batch where that leaves SMs without a CTA otherwise
+  const int groups = kThreads / G;
+  const int batches = T >= int64_t(groups) * kFwdRows * kFwdMaxBatches * ce::sm_count() * 8 ? kFwdMaxBatches : 1;
+  const int64_t per_cta = int64_t(groups) * kFwdRows * batches, grid = (T + per_cta - 1) / per_cta;
   NM_REQUIRE(grid <= INT_MAX, "embed_fwd: too many rows for one launch");
   auto kern = bf16 ? k_embed_fwd<true> : k_embed_fwd<false>;
-  kern<<<unsigned(grid), kThreads, 0, st>>>(table, tokens, out, scale, T, D, V, G);
+  kern<<<unsigned(grid), kThreads, 0, st>>>(table, tokens, out, scale, T, D, V, G, batches);
   NM_CUDA(cudaGetLastError());
 }
 

@@ -24,6 +24,7 @@ def test_forward_refusals(lib):  # noqa: F811
     refuse("cannot be negative", T=-1)
     refuse("multiple of 8", D=12)
     refuse("multiple of 8", D=0)
+    refuse("D <= 65536", D=65544)
     refuse("vocabulary size", V=0)
     refuse("required", table=None)
     refuse("required", tokens=None)
@@ -45,6 +46,7 @@ def test_backward_refusals(lib):  # noqa: F811
     refuse("storage 0 (f32) or 1 (bf16)", dtype=-1)
     refuse("cannot be negative", T=-4)
     refuse("multiple of 8", D=20)
+    refuse("D <= 65536", D=131072)
     refuse("vocabulary size", V=-3)
     refuse("required", dy=None)
     refuse("required", tokens=None)

@@ -317,6 +317,30 @@ def test_nothing_outside_the_buffers_is_written(fwd):
     assert status.value == 0
 
 
+def test_no_gradient_asked_of_a_full_call():
+    """forward_only = 0 with neither dx nor dw: the losses of a forward-only call, in a workspace with a logits store."""
+    from gpu_common import lib, nmce
+    T, D, V, K = 300, 64, 5, 40                                  # more entries than vocabulary
+    c = _case(T, D, V, K, tau=1.0)
+    ev, _, _ = _run(c, soft=0.5, hard=0.5, fwd=True)
+    ws = torch.empty(lib().nm_ce_distill_workspace_bytes(T, D, V, K, 128, 0), dtype=torch.uint8, device="cuda")
+    out = torch.empty(3, T, device="cuda")
+    p = nmce.ptr
+    lib().nm_ce_distill(0, p(c["x"]), p(c["w"]), p(c["ids"]), p(c["t"]), None, p(c["targets"]), p(c["weight"]), None, 1.0, 0.5,
+                        0.5, p(out[0]), p(out[1]), p(out[2]), None, None, 0, None, 0, T, D, V, K, 128, BIG_NEG, p(ws),
+                        ws.numel(), None)
+    assert all(torch.equal(a, b) for a, b in zip(out, ev))
+
+
+def test_soft_and_hard_alone():
+    c = _case(150, 128, 900, 9, tau=2.0)
+    for soft, hard in ((0.0, 1.0), (2.5, 0.0), (0.0, 0.0)):
+        out, dx, dw = _run(c, soft=soft, hard=hard)
+        _check(c, soft, hard, out, dx, dw)
+        if soft == hard == 0.0:
+            assert bool((dx == 0).all()) and bool((dw == 0).all())
+
+
 def test_no_rows():
     from gpu_common import lib, nmce
     assert lib().nm_ce_distill(0, *[None] * 8, 1.0, 1.0, 0.0, *[None] * 5, 0, None, 0, 0, 64, 100, 4, 128, 0, None, 0, None) == 0

@@ -249,3 +249,44 @@ def test_nothing_outside_the_buffers_is_written():
     lib.nm_embed_bwd(0, ptr(dy), ptr(tokens), ptr(out[1]), 1.0, 0, T, D, V, ptr(ws), need, None)
     _check_bwd(dy, tokens, V, 1.0, None, out[1:-1])
     assert bool((ws[need:] == 0x5A).all()) and bool((out[0] == 9).all()) and bool((out[-1] == 9).all())
+
+
+@pytest.mark.parametrize("T", [5, 5000])
+def test_no_token_inside_the_vocabulary(T):
+    V, D = 100, 64
+    dy = torch.full((T, D), float("nan"), device="cuda")          # rows that do not count are not read
+    tokens = torch.where(torch.arange(T, device="cuda") % 2 == 0, -1, V).int()
+    assert bool((_bwd(dy, tokens, V, 1.0) == 0).all())
+    before = torch.randn(V, D, device="cuda")
+    assert torch.equal(_bwd(dy, tokens, V, 1.0, before), before)
+    tokens[3] = 7
+    dy[3] = 2.0
+    got = _bwd(dy, tokens, V, 1.5)
+    assert bool((got[7] == 3).all()) and float(got.abs().sum()) == 3 * D
+
+
+@pytest.mark.parametrize("add", [False, True])
+def test_a_gradient_that_is_only_16_byte_aligned(add):
+    """Rows of the gradient that do not start on 32 bytes take the narrower stores: the same bits."""
+    lib, p = _lib()
+    T, D, V = 3000, 72, 500
+    g = torch.Generator(device="cuda").manual_seed(8)
+    dy = torch.randn(T, D, generator=g, device="cuda").bfloat16()
+    tokens = torch.randint(-1, 40, (T,), generator=g, device="cuda").int()
+    before = torch.randn(V, D, generator=g, device="cuda")
+    want = _bwd(dy, tokens, V, 2.0, before if add else None)
+    room = torch.full((V * D + 8,), 9.0, device="cuda")
+    out = room[4:4 + V * D].view(V, D)
+    out.copy_(before)
+    assert out.data_ptr() % 32 == 16
+    ws = torch.empty(lib.nm_embed_bwd_workspace_bytes(T, D, V), dtype=torch.uint8, device="cuda")
+    lib.nm_embed_bwd(1, p(dy), p(tokens), p(out), 2.0, int(add), T, D, V, p(ws), ws.numel(), None)
+    assert torch.equal(out, want) and bool((room[:4] == 9).all()) and bool((room[-4:] == 9).all())
+
+
+def test_widest_rows():
+    T, D, V = 40, 65536, 6
+    g = torch.Generator(device="cuda").manual_seed(2)
+    dy = torch.randn(T, D, generator=g, device="cuda")
+    tokens = torch.randint(0, V, (T,), generator=g, device="cuda").int()
+    _check_bwd(dy, tokens, V, 1.0, None, _bwd(dy, tokens, V, 1.0))
