@@ -647,7 +647,9 @@ void launch_distill_dgrad(const DistillDgradArgs& a, cudaStream_t st) {
   p.k_part = (kb + a.shares - 1) / a.shares;
   p.k_parts = a.shares;
   NM_REQUIRE((p.k_parts - 1) * p.k_part < kb, "distillation: an empty share of the dX contraction");
-  const CUtensorMap ta = tmap_kmajor(a.n, a.rows, a.ldn, a.ldn, BM);   // spans both terms
+  // spans both terms; with hi alone every other 128 bytes, and fetching them by 256 would read lo as well
+  const CUtensorMap ta = make_tmap(a.n, uint64_t(a.ldn), uint64_t(a.rows), a.ldn, BK, BM, false, 128,
+                                   p.k_terms == 2 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
   const CUtensorMap tb = tmap_mn_b(a.w, a.V, a.D, a.D, p.b_3d, 1);
   launch_n<kEpiDx, false, true, 1, true>(ta, tb, ta, p, st, 0);
 }
