@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
 }
 
 // Student logits of the listed ids for a call that stores none: one f32 dot product of x_t and W[id] each. A warp takes four
-// entries of a row at a time, a lane every 32nd 16-byte piece of the two rows.
+// entries of a row at a time, a lane every 32nd 16-byte piece of the two rows. 2125 x 16 entries of width 512: 11 us of
+// latency, where storing and gathering the logits would move a gigabyte.
 constexpr int kDotEntries = 4;
 __global__ void __launch_bounds__(256) k_distill_dots(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
                                                       const int32_t* __restrict__ ids, const float* __restrict__ weight,
@@ -243,7 +244,8 @@ __global__ void __launch_bounds__(256) k_distill_dots(const __nv_bfloat16* __res
 }
 
 // f32 logits -> the two-term gradient in place, then the listed elements on top. A CTA takes kSegment columns of a row; eight
-// lanes of a warp hold the 64 logits of a block before any of them is overwritten. Bound by HBM: 4 bytes in, 4 out.
+// lanes of a warp hold the 64 logits of a block before any of them is overwritten. Bound by HBM: 4 bytes in, 4 out,
+// 8192 x 128256 in 1.21 ms (6.9 TB/s).
 constexpr int kSegment = 4096, kGradThreads = 256;
 struct TwoTerm {
   uint16_t hi, lo;
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(kGradThreads) k_distill_grad(float* store, int
   }
 }
 
-// dx = round(scale * sum of the shares in order (+ dx))
+// dx = round(scale * sum of the shares in order (+ dx)); bound by HBM and launch latency (2125 x 1024, two shares: 6 us)
 __global__ void __launch_bounds__(256) k_distill_dx_join(const float* __restrict__ part, int shares, int64_t n8,
                                                          const float* __restrict__ scale, __nv_bfloat16* dx, bool add) {
   using namespace nm::ew;

@@ -2,9 +2,10 @@
 // adds the gradient below into the buffer that the fused CE accumulates dW in).
 //   forward   y[t, :] = round(scale * E[token_t, :])             a token outside [0, V) gives a row of zeros
 //   backward  dE[v, :] (+)= scale * sum_{t: token_t = v} dy[t, :]  in f32; a token outside [0, V) contributes nothing
-// The backward has no floating-point atomics: tokens are sorted by a stable radix sort, a run of equal tokens is summed
-// in ascending t, and long runs are cut at places that depend on the sorted tokens alone, so that the same call gives the
-// same bits. Counterpart in the reference: src/kernels/elementwise/embed.cu.
+// No sum of the backward depends on an order of atomics: tokens are sorted by a stable radix sort, a run of equal tokens is
+// summed in ascending t, long runs are cut at places that depend on the sorted tokens alone, and a call that adds makes one
+// addition per element, so that the same call gives the same bits. Counterpart in the reference:
+// src/kernels/elementwise/embed.cu.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -78,7 +79,8 @@ using nm::ptx::release_next;
 // ------------------------------------------------------------------------------------------------ forward
 // G threads side by side on a row (eight elements each); a row group takes `batches` times kFwdRows consecutive rows, the
 // loads of a batch in flight while the one before it is stored. Bound by HBM: the output is written once, past the L2 (the
-// frequent rows of the table are read from there again and again).
+// frequent rows of the table are read from there again and again). 131072 x 2048 bf16, ids falling as 1 / rank (35 thousand
+// distinct rows): 122 us, 5.6 TB/s; four rows once per group 128 us, eight 134 us, two 163 us.
 constexpr int kFwdRows = 4, kFwdMaxBatches = 4;
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads) k_embed_fwd(const void* __restrict__ table, const int32_t* __restrict__ tokens,
@@ -127,7 +129,8 @@ __global__ void __launch_bounds__(kThreads) k_embed_fwd(const void* __restrict__
 // One cluster of up to sixteen CTAs sorts the positions of a section by token: a least-significant-digit radix sort, nine
 // bits a pass, whose items never leave shared memory between passes (a pass scatters them into the other CTAs' shared
 // memory). CTA r holds the items [r * per, (r + 1) * per). Within a pass a warp ranks its items of equal digit by
-// match.any, 32 consecutive items at a time, which keeps the sort stable.
+// match.any, 32 consecutive items at a time, which keeps the sort stable. Bound by latency (shared-memory scans, two cluster
+// barriers a pass): 131072 tokens of 17 bits 43 us on 16 CTAs, 75 us on 8; beside the zeroing it costs nothing.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kDigitBits = 9, kDigits = 1 << kDigitBits;
 constexpr int kMaxCluster = 16, kMaxPerThread = 8, kPosBits = 17;
 constexpr int64_t kSection = int64_t(kMaxCluster) * kSortThreads * kMaxPerThread;   // 131072 tokens
@@ -160,7 +163,8 @@ inline __host__ __device__ uint32_t sort_smem_bytes(int per) {
 }
 
 // A short section (at most kRankMax tokens) needs no radix passes: the place of a token in the sorted order is the number
-// of tokens that are smaller, or equal and earlier. 32 positions per CTA, one per lane; warp w counts over the w-th eighth
+// of tokens that are smaller, or equal and earlier (2125 tokens: a few us of latency against 12 us for the radix sort).
+// 32 positions per CTA, one per lane; warp w counts over the w-th eighth
 // of the tokens, which lie in shared memory.
 constexpr int kRankMax = 4096, kRankWarps = kThreads / 32;
 __global__ void __launch_bounds__(kThreads) k_embed_rank(const SortParams p) {
@@ -196,7 +200,8 @@ __global__ void __launch_bounds__(kThreads) k_embed_rank(const SortParams p) {
 // Zeroes the rows that no token of the section names (the larger part of the writes of an overwriting call whose
 // vocabulary is larger than the section). It needs the tokens, not their order, so it runs beside the sort: it does not wait
 // for the launch before it until it has done its work. The vocabulary is dealt to the CTAs (a power of two of them) in
-// blocks of eight rows, because frequent ids lie together; a CTA marks the tokens of its share, then writes.
+// blocks of eight rows, because frequent ids lie together; a CTA marks the tokens of its share (10 us for 131072 tokens), then
+// writes. Bound by HBM: 850 MB in 137 us; dealt in contiguous ranges 148 us.
 constexpr int kZeroThreads = 1024, kZeroSlab = 65536;   // rows whose presence a CTA marks at a time (8 KiB of bits)
 struct ZeroParams {
   const int32_t* tokens;
@@ -383,7 +388,8 @@ __device__ __forceinline__ int first_owned(const Key& key, int b, int win, int V
 
 // A thread's pieces of the rows to come travel through its own slots of a ring in shared memory (cp.async, no barrier:
 // nobody else reads them), 64 KiB in flight per CTA: what a window waits for is a few round trips, and registers do not
-// limit how many rows are on their way.
+// limit how many rows are on their way. Bound by HBM: 131072 x 2048 bf16 into 35 thousand rows 128 us (740 MB, 5.8 TB/s);
+// with loads into registers 175 us.
 template <bool BF16>
 struct Ring {
   static constexpr int kGroups = 4;                        // commit groups in flight
@@ -527,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_embed_reduce(const ReduceParams
 // Joins the pieces of the listed cut runs: slot 1 of the window the run begins in, then slot 0 of the windows after it, in
 // that order. A job is 128 columns of one run and belongs to a warp; a run of more than kJoinAlone pieces is summed by all
 // warps of the CTA together (pieces dealt to the warps, their sums added in warp order), so that what the launch takes is
-// a few round trips whatever the longest run.
+// a few round trips whatever the longest run: 12 us for the 131072-token case, 26 us with a CTA per job.
 constexpr int kJoinCols = 128, kJoinWarps = kThreads / 32, kJoinAlone = 16;
 struct JoinJob {
   int win, second, pieces, col, key;

@@ -10,8 +10,9 @@
 // backward forms x_out again from x_in, branch and gate instead of reading it: bit for bit the stored one, because both
 // directions share outer() below, and 2 bytes per element less.
 // sigmoid(g) = r = 1 / (1 + e) and 1 - sigmoid(g) = e r with e = exp(-g): no cancellation at either end.
-// Row groups and batch ring as in ew_rows.cuh. What bounds them is HBM (10 and 16 bytes per element in bf16 with a gate per
-// element).
+// Row groups and batch ring as in ew_rows.cuh, a CTA per part of consecutive rows. What bounds them is HBM (10 and 16 bytes
+// per element in bf16 with a gate per element), and under the board's power cap, at 1.7 GHz, the issue slots. Forward,
+// 65536 x 2048: 217 us (6.2 TB/s), 231 us under the cap; the backward's figures stand at its kernel.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -308,19 +309,10 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
   if (threadIdx.x == 0 && *abort_flag) __nanosleep(200000);   // an expired wait: let copies in flight land first
 }
 
-// The second row sum needs the first (sum(branch p) is taken over m, which needs sum(x_out a)), but m is linear in it,
-// m = h + c x_out with h = dx_out + r_n a and c = -r_n^3 sum(x_out a) / D, so
-//   sum(u m) = sum(u h) + c sum(u x_out),   u = sigmoid(gate) y,
-// and all sums are taken in the first pass, with one barrier per row. sum(branch p) = sum(u m) / r_p; for a gate per token
-// sum(m y) is the same sum without the (constant) gate. x_out as stored and h stay in registers for the second pass, the
-// gate is evaluated again; the gains lie in shared memory (of ones where the call has none). Beside a ring that takes
-// nearly all of the SM's memory a spilled register is read back from L2, so the registers decide the form. Measured for
-// 65536 x 2048 bf16 with a gate per element (floor 328 us at the copy rate): 811 us with the gate's two parts kept and eight
-// columns at a time (spills), 414 us as quads without spills, 396 us with scalar instead of packed f32x2 arithmetic, 353 us
-// with the next batch fetched before a batch is worked on (6.08 TB/s). Sixteen columns per thread beat eight (439 us).
 // The gain sums of a CTA's row groups, added in group order, as one row of the partial buffer (smem: 256 float4).
 template <int N>
-__device__ __forceinline__ void write_quad_partial(const Two (&dg)[N][2], const RowGroup& rg, int quads, float* smem, float* out_row) {
+__device__ __forceinline__ void write_quad_partial(const Two (&dg)[N][2], const RowGroup& rg, int quads, float* smem,
+                                                   float* out_row) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int at = first_quad<N>(rg) + 32 * j;
@@ -339,6 +331,16 @@ __device__ __forceinline__ void write_quad_partial(const Two (&dg)[N][2], const 
   }
 }
 
+// The second row sum needs the first (sum(branch p) is taken over m, which needs sum(x_out a)), but m is linear in it,
+// m = h + c x_out with h = dx_out + r_n a and c = -r_n^3 sum(x_out a) / D, so
+//   sum(u m) = sum(u h) + c sum(u x_out),   u = sigmoid(gate) y,
+// and all sums are taken in the first pass, with one barrier per row. sum(branch p) = sum(u m) / r_p; for a gate per token
+// sum(m y) is the same sum without the (constant) gate. x_out as stored and h stay in registers for the second pass, the
+// gate is evaluated again; the gains lie in shared memory (of ones where the call has none). Beside a ring that takes
+// nearly all of the SM's memory a spilled register is read back from L2, so the registers decide the form. Measured for
+// 65536 x 2048 bf16 with a gate per element (floor 328 us at the copy rate): 811 us with the gate's two parts kept and eight
+// columns at a time (spills), 414 us as quads without spills, 396 us with scalar instead of packed f32x2 arithmetic, 353 us
+// with the next batch fetched before a batch is worked on (6.08 TB/s). Sixteen columns per thread beat eight (439 us).
 template <bool BF16, int PP, int GATE>
 __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gated_bwd(const TailParams p) {
   using namespace nm::ptx;
@@ -402,7 +404,8 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
     if constexpr (GATE == kTokenGate) tgate = gate_of(two(mine.gate, mine.gate));
     mine = scalars_of(r0 + rg.groups);
     const Two rn = two(r_n, r_n), rp = two(r_p, r_p);
-    if (threadIdx.x == 0 && ahead < tr.rows) {   // (as early as can be: two stages are all that fit) the slot of the batch before takes the batch stages - 1 ahead
+    // the slot of the batch before takes the batch stages - 1 ahead, as early as can be: two stages are all that fit
+    if (threadIdx.x == 0 && ahead < tr.rows) {
       const int prev = s == 0 ? p.stages - 1 : s - 1;
       mbar_wait(tr.ring.empty + 8u * prev, s == 0 ? phase ^ 1u : phase, abort_flag, p.status, kErrProducerWait);
       tr.fetch(p, prev, ahead, rg.groups);
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
 }
 
 // out[a][col] = sum over the parts, a the three gains (blockIdx.y): 32 columns per CTA, the parts dealt to 32 row lanes
-// whose sums are added in lane order.
+// whose sums are added in lane order. Bound by latency: ten loads in a row, some 5 us.
 struct GainSums {
   const float* part[3];
   float* out[3];
