@@ -359,7 +359,7 @@ DistillRegions layout(const DistillHeadShape& s, void* base) {
     r.pval = arena.take<float>(rows * uint64_t(s.K + 1));
     r.ldS = round_up(s.V, 64);
     r.store = arena.take<float>(rows * uint64_t(r.ldS));
-    r.dxpart = arena.take<float>(std::min<uint64_t>(32768, 16 * rows) * uint64_t(s.D));
+    r.dxpart = arena.take<float>(std::min<uint64_t>(kMaxDxShareRows, kMaxDxShares * rows) * uint64_t(s.D));
   }
   r.bytes = arena.bytes();
   return r;

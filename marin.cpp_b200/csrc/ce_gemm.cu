@@ -618,14 +618,14 @@ void launch_distill_logits(const DistillLogitsArgs& a, cudaStream_t st) {
 }
 
 // Shares of the dX contraction: one CTA per tile leaves SMs idle when a call has few tiles, or a last wave with few of them.
-// Of up to 16 shares the one with the fewest K blocks per SM is taken, a share counting 24 blocks more for its epilogue
-// and the reading of its sums; the sums take at most 32768 x D f32.
+// Of up to kMaxDxShares shares the one with the fewest K blocks per SM is taken, a share counting 24 blocks more for its epilogue
+// and the reading of its sums; the sums take at most kMaxDxShareRows x D f32.
 int distill_dgrad_shares(int rows, int D, int V) {
   const int64_t tiles = int64_t((rows + BM - 1) / BM) * ((D + BN - 1) / BN), sms = sm_count();
   const int64_t kb = (V + BK - 1) / BK * (rows <= kTwoTermDxRows ? 2 : 1);
   int best = 1;
   int64_t least = INT64_MAX;
-  for (int s = 1; s <= 16 && int64_t(s) * rows <= 32768 && s <= kb; ++s) {
+  for (int s = 1; s <= kMaxDxShares && int64_t(s) * rows <= kMaxDxShareRows && s <= kb; ++s) {
     const int64_t per = (kb + s - 1) / s;
     if ((kb + per - 1) / per != s) continue;   // a share would be empty
     const int64_t cost = (tiles * s + sms - 1) / sms * (per + (s > 1 ? 24 : 0));

@@ -192,7 +192,7 @@ void launch_distill_logits(const DistillLogitsArgs& a, cudaStream_t st);
 //       reads W from HBM for longer than either form computes, and both terms are taken.
 //   dW: both terms; the accumulator is drained into dw (f32) after at most kDrainRows rows, because the tensor core adds to
 //       it with truncation (measured: the relative error of a contraction of length K grows as 1e-9 K).
-constexpr int kDrainRows = 1152, kTwoTermDxRows = 128;
+constexpr int kDrainRows = 1152, kTwoTermDxRows = 128, kMaxDxShares = 16, kMaxDxShareRows = 32768;
 struct DistillDgradArgs {
   const void* n; int64_t ldn; const void* w;
   int rows, D, V;

@@ -356,6 +356,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
   const int quads = p.D / 4, first = first_quad<N>(rg);
   const bool post = p.g_post != nullptr, carried = p.dx_out != nullptr;
   constexpr int kGateOp = 3, kCarriedOp = GATE == kElementGate ? 4 : 3;
+  release_next();
   TailRing<BF16> tr;
   tr.begin(ring_raw, p, &abort_word);
   int ahead = 0;
@@ -534,6 +535,7 @@ struct GainSums {
 };
 __global__ void __launch_bounds__(1024) k_gated_gain_sums(const GainSums p) {
   __shared__ float red[32][33];
+  nm::ptx::after_previous();
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), lane_row = threadIdx.x >> 5;
   const float* part = p.part[blockIdx.y];
   float s = 0.f;
@@ -689,8 +691,7 @@ void gated_tail_bwd(bool bf16, int gate_kind, const void* dx_out, const void* da
   if (n > 0) {
     NM_REQUIRE(ce::device_arch() >= 100, "gated tail: this library holds sm_100a code only");
     gs.parts = int(p.parts), gs.D = D;   // no rows: no parts, the gradient of nothing
-    k_gated_gain_sums<<<dim3(unsigned((D + 31) / 32), unsigned(n)), 1024, 0, st>>>(gs);
-    NM_CUDA(cudaGetLastError());
+    ce::launch_after(k_gated_gain_sums, dim3(unsigned((D + 31) / 32), unsigned(n)), 1024, 0, st, gs);
   }
 }
 
