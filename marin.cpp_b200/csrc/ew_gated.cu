@@ -244,14 +244,20 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
       return r;
     };
     Two rp = two(1.f, 1.f);
+    Two bb[N][2];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (!(on_row && first + 32 * j < quads)) continue;
+      const Q b = quad(0, j);
+      bb[j][0] = b.pair(0), bb[j][1] = b.pair(1);
+    }
     if (post) {   // uniform over the CTA
       Two sbb = two(0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         if (!(on_row && first + 32 * j < quads)) continue;
-        const Q b = quad(0, j);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) sbb = fma(b.pair(q), b.pair(q), sbb);
+        for (int q = 0; q < 2; ++q) sbb = fma(bb[j][q], bb[j][q], sbb);
       }
       float sum[1] = {both(sbb)};
       group_sum<1>(sum, rg, red, flip);
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (!(on_row && first + 32 * j < quads)) continue;
-      const Q b = quad(0, j), x = quad(1, j);
+      const Q x = quad(1, j);
       Q g;
       if constexpr (GATE == kElementGate) g = quad(2, j);
       Two v[2];
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
       for (int q = 0; q < 2; ++q) {
         Two on = token_on;
         if constexpr (GATE == kElementGate) on = gate_open(g.pair(q));
-        v[q] = outer<GATE>(mul(b.pair(q), rp), gp[j].pair(q), on, x.pair(q), sc[j].pair(q));
+        v[q] = outer<GATE>(mul(bb[j][q], rp), gp[j].pair(q), on, x.pair(q), sc[j].pair(q));
       }
       xo[j].round(v[0], v[1]);
       xo[j].to_global(static_cast<uint8_t*>(p.x_out) + out0 + 32 * j * int(Q::kBytes));
