@@ -28,14 +28,43 @@
 namespace nm::ew {
 namespace {
 
-// Two neighbouring f32 values, each operation individually rounded. Plain scalar instructions: the same kernels on the packed
-// f32x2 pipe (ew_rows.cuh) executed as many instructions and took 414 us instead of 396 us (backward, 65536 x 2048).
+// Two neighbouring f32 values, each operation individually rounded: the packed f32x2 form (fma2, mul2) and the plain one give
+// the same bits. Written as one asm block each: with the values held as 64-bit registers between the operations (ew_rows.cuh)
+// the moves that put single results side by side ate the gain. Backward, 65536 x 2048: 279 million warp instructions with
+// plain arithmetic, 243 million packed (390 -> 387 us under the power cap, 349 us at full clock either way: HBM).
 struct Two {
   float x, y;
 };
 __device__ __forceinline__ Two two(float a, float b) { return Two{a, b}; }
 __device__ __forceinline__ Two mul(Two a, Two b) { return Two{__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)}; }
 __device__ __forceinline__ Two fma(Two a, Two b, Two c) { return Two{fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)}; }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("{\n\t"
+      ".reg .b64 a, b, c;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t"
+      "}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("{\n\t"
+      ".reg .b64 a, b;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t"
+      "}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 __device__ __forceinline__ Two two_of(uint32_t w) { return Two{lo_f32(w), hi_f32(w)}; }
 
 enum GateKind : int { kNoGate = 0, kTokenGate = 1, kElementGate = 2 };
@@ -128,7 +157,7 @@ __device__ __forceinline__ Gate2 gate_of(Two g) {
 template <int GATE>
 __device__ __forceinline__ Two outer(Two n, Two gp, Two on, Two x, Two s) {
   const Two y = mul(n, gp);
-  return fma(s, x, GATE == kNoGate ? y : mul(on, y));
+  return fma2(s, x, GATE == kNoGate ? y : mul(on, y));
 }
 __device__ __forceinline__ float both(Two v) { return v.x + v.y; }
 
@@ -257,7 +286,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
       for (int j = 0; j < N; ++j) {
         if (!(on_row && first + 32 * j < quads)) continue;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) sbb = fma(bb[j][q], bb[j][q], sbb);
+        for (int q = 0; q < 2; ++q) sbb = fma2(bb[j][q], bb[j][q], sbb);
       }
       float sum[1] = {both(sbb)};
       group_sum<1>(sum, rg, red, flip);
@@ -284,7 +313,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
       xo[j].round(v[0], v[1]);
       xo[j].to_global(static_cast<uint8_t*>(p.x_out) + out0 + 32 * j * int(Q::kBytes));
 #pragma unroll
-      for (int q = 0; q < 2; ++q) sxx = fma(xo[j].pair(q), xo[j].pair(q), sxx);
+      for (int q = 0; q < 2; ++q) sxx = fma2(xo[j].pair(q), xo[j].pair(q), sxx);
     }
     float sum[1] = {both(sxx)};
     group_sum<1>(sum, rg, red1, flip1);
@@ -345,8 +374,8 @@ __device__ __forceinline__ void write_quad_partial(const Two (&dg)[N][2], const 
 // gate is evaluated again; the gains lie in shared memory (of ones where the call has none). Beside a ring that takes
 // nearly all of the SM's memory a spilled register is read back from L2, so the registers decide the form. Measured for
 // 65536 x 2048 bf16 with a gate per element (floor 328 us at the copy rate): 811 us with the gate's two parts kept and eight
-// columns at a time (spills), 414 us as quads without spills, 396 us with scalar instead of packed f32x2 arithmetic, 353 us
-// with the next batch fetched before a batch is worked on (6.08 TB/s). Sixteen columns per thread beat eight (439 us).
+// columns at a time (spills), 414 us as quads without spills, 353 us with plain arithmetic instead of
+// packed 64-bit registers and the next batch fetched before a batch is worked on (6.1 TB/s). Sixteen columns per thread beat eight (439 us).
 template <bool BF16, int PP, int GATE>
 __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gated_bwd(const TailParams p) {
   using namespace nm::ptx;
@@ -447,10 +476,10 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
         for (int q = 0; q < 2; ++q) {
           Two on = tgate.on;
           if constexpr (GATE == kElementGate) on = gate_open(g.pair(q));
-          const Two n = mul(b.pair(q), rp);
+          const Two n = mul2(b.pair(q), rp);
           v[q] = outer<GATE>(n, gp.pair(q), on, x.pair(q), sc.pair(q));
-          u[q] = mul(n, gp.pair(q));
-          if constexpr (GATE == kElementGate) u[q] = mul(on, u[q]);
+          u[q] = mul2(n, gp.pair(q));
+          if constexpr (GATE == kElementGate) u[q] = mul2(on, u[q]);
         }
       }
       xo[j].round(v[0], v[1]);
@@ -461,12 +490,12 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
       const GainQ gn = gain(0, j);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const Two xoq = xo[j].pair(q), a = mul(gn.pair(q), da.pair(q));
-        sxa = fma(xoq, a, sxa);
-        h[j][q] = fma(rn, a, dxo.pair(q));
-        dgn[j][q] = fma(da.pair(q), mul(xoq, rn), dgn[j][q]);
-        suh = fma(u[q], h[j][q], suh);
-        sux = fma(u[q], xoq, sux);
+        const Two xoq = xo[j].pair(q), a = mul2(gn.pair(q), da.pair(q));
+        sxa = fma2(xoq, a, sxa);
+        h[j][q] = fma2(rn, a, dxo.pair(q));
+        dgn[j][q] = fma2(da.pair(q), mul2(xoq, rn), dgn[j][q]);
+        suh = fma2(u[q], h[j][q], suh);
+        sux = fma2(u[q], xoq, sux);
       }
     }
     float sums[3] = {both(sxa), both(suh), both(sux)};
@@ -495,21 +524,21 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
       Two vx[2], vg[2], vb[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const Two m = fma(c_n, xo[j].pair(q), h[j][q]);
-        vx[q] = mul(m, sc.pair(q));
-        dsc[j][q] = fma(m, x.pair(q), dsc[j][q]);
-        Two t = mul(m, rp);   // t r_p from here on: its products with the branch are those of t with the normalised branch
-        if constexpr (GATE == kTokenGate) t = mul(t, tgate.on);
+        const Two m = fma2(c_n, xo[j].pair(q), h[j][q]);
+        vx[q] = mul2(m, sc.pair(q));
+        dsc[j][q] = fma2(m, x.pair(q), dsc[j][q]);
+        Two t = mul2(m, rp);   // t r_p from here on: its products with the branch are those of t with the normalised branch
+        if constexpr (GATE == kTokenGate) t = mul2(t, tgate.on);
         Two off;
         if constexpr (GATE == kElementGate) {
           const Gate2 z = gate_of(g.pair(q));
-          t = mul(t, z.on);
+          t = mul2(t, z.on);
           off = z.off;
         }
-        dgp[j][q] = fma(t, b.pair(q), dgp[j][q]);
-        const Two pr = mul(gp.pair(q), t);
-        if constexpr (GATE == kElementGate) vg[q] = mul(mul(pr, b.pair(q)), off);
-        vb[q] = fma(c_p, b.pair(q), pr);
+        dgp[j][q] = fma2(t, b.pair(q), dgp[j][q]);
+        const Two pr = mul2(gp.pair(q), t);
+        if constexpr (GATE == kElementGate) vg[q] = mul2(mul2(pr, b.pair(q)), off);
+        vb[q] = fma2(c_p, b.pair(q), pr);
       }
       constexpr int kStep = 32 * int(Q::kBytes);
       Q o;
