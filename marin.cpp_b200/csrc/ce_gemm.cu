@@ -54,11 +54,12 @@ constexpr int two_term_smem_bytes() {
 }
 
 // ---------------------------------------------------------------------------------------------- the kernel
-// TWO (the distillation head's gradient contractions): A is the two-term gradient of ce_internal.hpp. dX (A K-major): K
-// block kb is the hi block kb, at column 128 kb, or with p.k_terms = 2 the blocks alternate between the terms; the tiles are dealt k_parts times, each time over its own k_part K blocks.
-// dW (A MN-major): a stage holds both terms of 64 rows and the 64 rows of x that they share; a CTA takes its tile k_parts
-// times in a row, k_part K blocks (counted per term) each, and its epilogue lets the additions of one part finish before it issues those of the next, so that
-// the order of additions is fixed.
+// TWO (the distillation head's gradient contractions): A is the two-term gradient of ce_internal.hpp. dX (A K-major): K block
+// kb is the hi block kb, at column 128 kb, or with p.k_terms = 2 the blocks alternate between the terms; the tiles are dealt
+// k_parts times, each time over its own k_part K blocks. dW (A MN-major): a stage holds both terms of 64 rows and the 64 rows
+// of x that they share (8192 x 2048 x 128256: 7.0 ms, with a stage per term 8.0 ms); a CTA takes its tile k_parts times in a
+// row, k_part K blocks (counted per term) each, and its epilogue lets the additions of one pass finish before it issues those
+// of the next, so that the order of additions is fixed. Bound by the tensor cores under the board's power cap.
 template <int EPI, bool A_MN, bool B_MN, int NCTA, bool TWO = false>
 __global__ void __launch_bounds__(kThreads, 1)
 k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -618,8 +619,9 @@ void launch_distill_logits(const DistillLogitsArgs& a, cudaStream_t st) {
 }
 
 // Shares of the dX contraction: one CTA per tile leaves SMs idle when a call has few tiles, or a last wave with few of them.
-// Of up to kMaxDxShares shares the one with the fewest K blocks per SM is taken, a share counting 24 blocks more for its epilogue
-// and the reading of its sums; the sums take at most kMaxDxShareRows x D f32.
+// The number with the fewest K blocks per SM is taken, a share counting 24 blocks more for its epilogue and the reading of its
+// sums (16 rows x 512, 8256 ids, the whole call: 1 share 128 us, 4 63 us, 8 and 16 46 to 55 us, 43 58 us); the sums take at
+// most kMaxDxShareRows x D f32.
 int distill_dgrad_shares(int rows, int D, int V) {
   const int64_t tiles = int64_t((rows + BM - 1) / BM) * ((D + BN - 1) / BN), sms = sm_count();
   const int64_t kb = (V + BK - 1) / BK * (rows <= kTwoTermDxRows ? 2 : 1);
