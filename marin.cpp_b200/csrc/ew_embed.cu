@@ -80,10 +80,10 @@ using nm::ptx::release_next;
 // G threads side by side on a row (eight elements each); a row group takes `batches` times kFwdRows consecutive rows, the
 // loads of a batch in flight while the one before it is stored. Bound by HBM: the output is written once, past the L2 (the
 // frequent rows of the table are read from there again and again). 131072 x 2048 bf16, ids falling as 1 / rank (35 thousand
-// distinct rows): 122 us, 5.6 TB/s; four rows once per group 128 us, eight 134 us, two 163 us.
-constexpr int kFwdRows = 4, kFwdMaxBatches = 4;
+// distinct rows): 117 us, 5.8 TB/s; batches of three rows 118 us, of four 122 us, one batch of four rows per group 128 us.
+constexpr int kFwdRows = 2, kFwdMaxBatches = 8;
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads) k_embed_fwd(const void* __restrict__ table, const int32_t* __restrict__ tokens,
+__global__ void __launch_bounds__(kThreads, BF16 ? 6 : 4) k_embed_fwd(const void* __restrict__ table, const int32_t* __restrict__ tokens,
                                                         void* __restrict__ out, float scale, int64_t T, int D, int V, int G,
                                                         int batches) {
   __shared__ int32_t tok_s[kThreads / 32 * kFwdRows * kFwdMaxBatches];
