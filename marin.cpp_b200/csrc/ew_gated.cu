@@ -8,11 +8,11 @@
 // gate (per token or per element), s and g_post are optional. f32 inside, one rounding per stored output (the accurate
 // policy of the sandwich tail); x_out is what the residual stream holds, so the next norm reads its rounded values. The
 // backward forms x_out again from x_in, branch and gate instead of reading it: bit for bit the stored one, because both
-// directions share outer() below, and 2 bytes per element less.
+// directions share through() below, and 2 bytes per element less.
 // sigmoid(g) = r = 1 / (1 + e) and 1 - sigmoid(g) = e r with e = exp(-g): no cancellation at either end.
 // Row groups and batch ring as in ew_rows.cuh, a CTA per part of consecutive rows. What bounds them is HBM (10 and 16 bytes
 // per element in bf16 with a gate per element), and under the board's power cap, at 1.7 GHz, the issue slots. Forward,
-// 65536 x 2048: 217 us (6.2 TB/s), 231 us under the cap; the backward's figures stand at its kernel.
+// 65536 x 2048: 231 us (5.8 TB/s), 250 us under the cap; the backward's figures stand at its kernel.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -31,13 +31,13 @@ namespace {
 // Two neighbouring f32 values, each operation individually rounded: the packed f32x2 form (fma2, mul2) and the plain one give
 // the same bits. Written as one asm block each: with the values held as 64-bit registers between the operations (ew_rows.cuh)
 // the moves that put single results side by side ate the gain. Backward, 65536 x 2048: 279 million warp instructions with
-// plain arithmetic, 243 million packed (390 -> 387 us under the power cap, 349 us at full clock either way: HBM).
+// plain arithmetic, 243 million packed (390 -> 387 us under the power cap, 349 us at full clock either way: HBM; before the
+// quotient below was rounded once). Forward, the same size: 232 -> 231 us, 251 -> 250 us under the cap.
 struct Two {
   float x, y;
 };
 __device__ __forceinline__ Two two(float a, float b) { return Two{a, b}; }
 __device__ __forceinline__ Two mul(Two a, Two b) { return Two{__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)}; }
-__device__ __forceinline__ Two fma(Two a, Two b, Two c) { return Two{fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)}; }
 __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
   Two r;
   asm("{\n\t"
@@ -138,11 +138,7 @@ __device__ __forceinline__ float rcp_approx(float a) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
   return r;
 }
-constexpr float kLog2e = 1.4426950408889634f;
-__device__ __forceinline__ float gate_open(float g) {   // e = inf gives 0: no limit needed
-  return rcp_approx(__fadd_rn(1.f, nm::ptx::ex2_approx(__fmul_rn(g, -kLog2e))));
-}
-__device__ __forceinline__ Two gate_open(Two g) { return two(gate_open(g.x), gate_open(g.y)); }
+constexpr float kLog2e = 1.4426950408889634f, kLargest = 3.402823466e38f;
 __device__ __forceinline__ Gate2 gate_of(Two g) {
   const Two e = two(nm::ptx::ex2_approx(gate_exponent(__fmul_rn(g.x, -kLog2e))),
                     nm::ptx::ex2_approx(gate_exponent(__fmul_rn(g.y, -kLog2e))));
@@ -152,12 +148,34 @@ __device__ __forceinline__ Gate2 gate_of(Two g) {
   return r;
 }
 
-// The value of x_out before it is rounded, two elements: s x + on (n gp). A part that the call leaves out is a factor of one
-// (exact), so nothing below branches on it. Both directions use this one form and get the same bits.
-template <int GATE>
-__device__ __forceinline__ Two outer(Two n, Two gp, Two on, Two x, Two s) {
-  const Two y = mul(n, gp);
-  return fma2(s, x, GATE == kNoGate ? y : mul(on, y));
+// What x_out is made of, s x + y / (1 + exp(-gate)), takes expf and a quotient rounded once: x_out is rounded to the storage
+// type, and in bf16 a value next to a tie lands a whole step (2^-8) away for a difference of 2^-24, which every sum over x_out
+// shows. With ex2.approx of a rounded product and rcp.approx the f32 sums stood up to 2e-5 from those of the formula's own f32
+// operations, now 3e-7 (12 % of the forward and 6 % of the backward under the power cap). The quotient is q = y r, r about the
+// reciprocal of 1 + exp(-gate), refined by its remainder. The gate stops at -87, where the quotient is as good as 0; a NaN
+// passes through. The remainder of an infinite y is inf - inf; INF makes it a number and the quotient infinite. The backward
+// does without: the row's rstd_next is 0 and 0 inf = NaN reaches all its gradients either way. A part that the call leaves out
+// is a factor of one (exact), so nothing branches on it. Both directions get the same bits from these.
+struct Opening {
+  Two a, r;   // -(1 + exp(-gate)), and about the reciprocal of 1 + exp(-gate)
+};
+__device__ __forceinline__ float exp_of_minus(float g) {
+  asm("max.NaN.f32 %0, %0, 0fC2AE0000;" : "+f"(g));
+  return expf(-g);
+}
+__device__ __forceinline__ Opening opening_of(Two g) {
+  const Two e = two(exp_of_minus(g.x), exp_of_minus(g.y));
+  Opening o;
+  o.a = fma2(e, two(-1.f, -1.f), two(-1.f, -1.f));
+  o.r = two(rcp_approx(-o.a.x), rcp_approx(-o.a.y));
+  return o;
+}
+template <bool INF = true>
+__device__ __forceinline__ Two through(Two y, const Opening& o) {   // y / (1 + exp(-gate))
+  const Two q = mul2(y, o.r);
+  Two rest = fma2(q, o.a, y);
+  if constexpr (INF) rest = two(fmaxf(rest.x, -kLargest), fmaxf(rest.y, -kLargest));
+  return fma2(rest, o.r, q);
 }
 __device__ __forceinline__ float both(Two v) { return v.x + v.y; }
 
@@ -236,6 +254,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
   const RowGroup rg = row_group(p.G);
   const int quads = p.D / 4, first = first_quad<N>(rg);
   const bool post = p.g_post != nullptr, scaled = p.res_scale != nullptr;
+  const float inv_d = 1.f / float(p.D);
   TailRing<BF16> tr;
   tr.begin(ring_raw, p, &abort_word);
   int ahead = 0;
@@ -250,7 +269,6 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
       if (scaled) sc[j].from_global(p.res_scale, first + 32 * j);
     }
   }
-  const float inv_d = 1.f / float(p.D);
   auto gate_scalar = [&](int r) {
     if constexpr (GATE == kTokenGate) return r < tr.rows ? scalar_of(p.gate, tr.row0 + r, BF16) : 0.f;
     else return 0.f;
@@ -260,9 +278,9 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
   uint32_t phase = 0;
   for (int r0 = rg.group; r0 < tr.rows + rg.group; r0 += rg.groups) {   // batches; this thread's row of the part is r0
     const bool on_row = r0 < tr.rows;
-    Two token_on = two(1.f, 1.f);
+    Opening token;
     if constexpr (GATE == kTokenGate) {
-      token_on = gate_open(two(gate_next, gate_next));
+      token = opening_of(two(gate_next, gate_next));
       gate_next = gate_scalar(r0 + rg.groups);
     }
     mbar_wait<true>(tr.ring.full + 8u * s, phase, abort_flag, p.status, kErrTransformWait);
@@ -306,9 +324,10 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
       Two v[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        Two on = token_on;
-        if constexpr (GATE == kElementGate) on = gate_open(g.pair(q));
-        v[q] = outer<GATE>(mul(bb[j][q], rp), gp[j].pair(q), on, x.pair(q), sc[j].pair(q));
+        Two u = mul2(mul2(bb[j][q], rp), gp[j].pair(q));
+        if constexpr (GATE == kTokenGate) u = through(u, token);
+        if constexpr (GATE == kElementGate) u = through(u, opening_of(g.pair(q)));
+        v[q] = fma2(sc[j].pair(q), x.pair(q), u);
       }
       xo[j].round(v[0], v[1]);
       xo[j].to_global(static_cast<uint8_t*>(p.x_out) + out0 + 32 * j * int(Q::kBytes));
@@ -335,7 +354,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 ? 2 : 1) k_gated_fwd(co
         for (int j = 0; j < N; ++j) {
           if (first + 32 * j >= quads) continue;
           Q o;
-          o.round(mul(gn[j].pair(0), mul(xo[j].pair(0), rn)), mul(gn[j].pair(1), mul(xo[j].pair(1), rn)));
+          o.round(mul2(gn[j].pair(0), mul2(xo[j].pair(0), rn)), mul2(gn[j].pair(1), mul2(xo[j].pair(1), rn)));
           o.to_global(static_cast<uint8_t*>(p.a_next) + out0 + 32 * j * int(Q::kBytes));
         }
       }
@@ -375,7 +394,8 @@ __device__ __forceinline__ void write_quad_partial(const Two (&dg)[N][2], const 
 // nearly all of the SM's memory a spilled register is read back from L2, so the registers decide the form. Measured for
 // 65536 x 2048 bf16 with a gate per element (floor 328 us at the copy rate): 811 us with the gate's two parts kept and eight
 // columns at a time (spills), 414 us as quads without spills, 353 us with plain arithmetic instead of
-// packed 64-bit registers and the next batch fetched before a batch is worked on (6.1 TB/s). Sixteen columns per thread beat eight (439 us).
+// packed 64-bit registers and the next batch fetched before a batch is worked on (6.1 TB/s); 364-370 us, 414-426 us under the
+// power cap, since the gate's quotient is rounded once. Sixteen columns per thread beat eight (439 us).
 template <bool BF16, int PP, int GATE>
 __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gated_bwd(const TailParams p) {
   using namespace nm::ptx;
@@ -437,7 +457,11 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
     const bool on_row = r0 < tr.rows;
     const float r_n = mine.r_n, r_p = mine.r_p;
     Gate2 tgate{two(1.f, 1.f), two(0.f, 0.f)};
-    if constexpr (GATE == kTokenGate) tgate = gate_of(two(mine.gate, mine.gate));
+    Opening token;
+    if constexpr (GATE == kTokenGate) {
+      tgate = gate_of(two(mine.gate, mine.gate));
+      token = opening_of(two(mine.gate, mine.gate));
+    }
     mine = scalars_of(r0 + rg.groups);
     const Two rn = two(r_n, r_n), rp = two(r_p, r_p);
     // the slot of the batch before takes the batch stages - 1 ahead, as early as can be: two stages are all that fit
@@ -474,12 +498,11 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
         const GainQ gp = gain(1, j), sc = gain(2, j);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          Two on = tgate.on;
-          if constexpr (GATE == kElementGate) on = gate_open(g.pair(q));
-          const Two n = mul2(b.pair(q), rp);
-          v[q] = outer<GATE>(n, gp.pair(q), on, x.pair(q), sc.pair(q));
-          u[q] = mul2(n, gp.pair(q));
-          if constexpr (GATE == kElementGate) u[q] = mul2(on, u[q]);
+          u[q] = mul2(mul2(b.pair(q), rp), gp.pair(q));
+          Two through_gate = u[q];
+          if constexpr (GATE == kTokenGate) through_gate = through<false>(u[q], token);
+          if constexpr (GATE == kElementGate) through_gate = u[q] = through<false>(u[q], opening_of(g.pair(q)));
+          v[q] = fma2(sc.pair(q), x.pair(q), through_gate);
         }
       }
       xo[j].round(v[0], v[1]);

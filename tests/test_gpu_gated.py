@@ -323,3 +323,31 @@ def test_status_word_stays_clean():
     word = ctypes.c_uint32(9)
     lib.nm_norm_bwd_device_status(None, ctypes.byref(word))
     assert word.value == 0
+
+
+@pytest.mark.parametrize("kind", [1, 2])
+@pytest.mark.parametrize("T,D", [(333, 520), (40, 2048)])
+def test_the_open_part_of_far_gates(kind, T, D):
+    """f32 without the post norm, gates of magnitude up to 80. Counted in half steps u: the product branch g_post 1, exp 2 ulp
+    (4 u), 1 + exp 1, the quotient 1 and a second-order rest, x_out's own rounding 1: under 9 u of |s x| + |open y|."""
+    s = _inputs(0, T, D, kind, False, True)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    s["gate"] = torch.rand(s["gate"].shape, generator=g, device="cuda") * 160 - 80
+    x_out = _fwd(0, kind, s)[0]
+    d = {k: v.double() for k, v in s.items() if v is not None}
+    carried = d["scale"] * d["x_in"]
+    through = torch.sigmoid(d["gate"][:, None] if kind == 1 else d["gate"]) * d["branch"]
+    _near("x_out", x_out, carried + through, 9 * U * (carried.abs() + through.abs()))
+
+
+@pytest.mark.parametrize("dtype", [1, 0])
+@pytest.mark.parametrize("kind", [1, 2])
+def test_an_infinite_branch_passes_the_gate(dtype, kind):
+    s = _inputs(dtype, 6, 264, kind, False, True)
+    s["branch"][1, 5], s["branch"][3, 260], s["branch"][4, 7] = float("inf"), float("-inf"), float("nan")
+    x_out, a_next, _, _ = _fwd(dtype, kind, s)
+    assert float(x_out[1, 5]) == float("inf") and float(x_out[3, 260]) == float("-inf") and bool(x_out[4, 7].isnan())
+    assert int(x_out.isfinite().logical_not().sum()) == 3
+    for row in (1, 3):      # the statistic of a row with an infinity is 0: its finite elements become 0
+        assert int((a_next[row] == 0).sum()) == 263 and int(a_next[row].isnan().sum()) == 1
+    assert bool(a_next[[0, 2, 5]].isfinite().all()) and bool(a_next[4].isnan().all())
