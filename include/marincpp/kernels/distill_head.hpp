@@ -10,7 +10,8 @@
 // With teacher_lse (log sum over the teacher's whole vocabulary of exp(. / tau)) the q_k keep their true mass and kl_t is the
 // listed part of the divergence. An entry whose id lies outside [0, V) is padding: its logit is not looked at. Ids may repeat
 // within a row (their masses add). A row without entries has no soft term, a row whose target lies outside [0, V) or equals
-// ignore_index no hard term, a row of weight 0 neither loss nor gradient.
+// ignore_index no hard term, a row of weight 0 neither loss nor gradient; its x must be finite all the same where dW is asked
+// for (0 x_t is taken, as in the fused head).
 // No counterpart in the reference, whose heads take hard targets only.
 #pragma once
 
