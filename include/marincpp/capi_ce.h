@@ -148,7 +148,7 @@ int nm_ce_sampled_head(int rounding, int logits_store, const void* x, const void
  *      against a teacher's listed logits [T, K] (ids outside [0, V) are padding), q their softmax at temperature tau, or with
  *      teacher_lse [T] (log sum exp(. / tau) over the teacher's whole vocabulary) their true masses; and its gradients
  *      dx [T, D] bf16 (accumulate_dx: added to) and dw [V, D] f32 (added to). x, w bf16, D % 8 == 0; teacher_dtype 0 f32,
- *      1 bf16; K 1 .. 512. NULL: teacher_lse, targets (when hard_weight is 0), kl_tok, lse (log sum exp(z / tau)),
+ *      1 bf16; K 1 .. 512; V and the rows of a chunk at most 2^30. NULL: teacher_lse, targets (when hard_weight is 0), kl_tok, lse (log sum exp(z / tau)),
  *      loss_partial, dx, dw, and grad_scale when both are NULL. dx may be x when it does not accumulate. forward_only != 0:
  *      no gradients, and a workspace without a logits store. Same bits for the same call and chunk_rows. workspace: 256-byte
  *      aligned, nm_ce_distill_workspace_bytes (0 on error) with the same arguments; word 0 is the wait status

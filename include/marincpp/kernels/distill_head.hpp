@@ -23,9 +23,9 @@ namespace nm {
 
 struct DistillHeadShape {
   int64_t T;             // rows in the call
-  int D, V;
+  int D, V;              // D a multiple of 8, V at most 2^30
   int K;                 // teacher entries per row, 1 .. 512
-  int chunk_rows;
+  int chunk_rows;        // min(T, chunk_rows) at most 2^30
   bool forward_only;     // no logits are stored: a much smaller workspace
 };
 

@@ -27,7 +27,7 @@ using nm::ew::warp_sum;
 using nm::ptx::ex2_approx;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxEntries = 512;
+constexpr int kMaxEntries = 512, kMaxExtent = 1 << 30;
 
 // What the rewrite of a row's logits needs: n = a_t 2^(z log2e / tau + e_t) + a_1 2^(z log2e + e_1) - (listed entries)
 struct alignas(16) DistillRow {
@@ -368,9 +368,11 @@ DistillRegions layout(const DistillHeadShape& s, void* base) {
 void require_shape(const DistillHeadShape& s) {
   NM_REQUIRE(s.T >= 0, "distillation: the row count T cannot be negative");
   NM_REQUIRE(s.D > 0 && s.D % 8 == 0, "distillation: D must be a positive multiple of 8 (rows are moved in 16-byte pieces)");
-  NM_REQUIRE(s.V > 0 && s.V <= INT32_MAX - 64, "distillation: the vocabulary size V must be positive");
+  // the two-term gradient is 2 V columns wide and its TMA coordinates are 32-bit
+  NM_REQUIRE(s.V > 0 && s.V <= kMaxExtent, "distillation: the vocabulary size V must be positive and at most 2^30");
   NM_REQUIRE(s.K >= 1 && s.K <= kMaxEntries, "distillation: 1 to 512 teacher entries per row");
   NM_REQUIRE(s.chunk_rows > 0, "distillation: chunk_rows must be positive");
+  NM_REQUIRE(std::min<int64_t>(s.T, s.chunk_rows) <= kMaxExtent, "distillation: at most 2^30 rows per chunk");
 }
 bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
