@@ -402,6 +402,11 @@ void distill_head(const DistillHeadShape& s, const DistillHeadArgs& a, void* ws,
              "distillation: x, w, dx and dw must be 16-byte aligned");
   NM_REQUIRE(aligned(a.teacher_ids, 4) && aligned(a.teacher_logits, dtype_size(a.teacher_dtype)),
              "distillation: teacher entries must be aligned to their size");
+  for (const void* p : {static_cast<const void*>(a.teacher_lse), static_cast<const void*>(a.targets),
+                        static_cast<const void*>(a.weight), static_cast<const void*>(a.grad_scale),
+                        static_cast<const void*>(a.loss_tok), static_cast<const void*>(a.kl_tok),
+                        static_cast<const void*>(a.lse), static_cast<const void*>(a.loss_partial)})
+    NM_REQUIRE(aligned(p, 4), "distillation: targets, weights, statistics and losses must be 4-byte aligned");
   NM_REQUIRE(ws != nullptr && aligned(ws, kArenaAlign), "distillation: a 256-byte aligned workspace is required");
   NM_REQUIRE(ws_bytes >= layout(s, nullptr).bytes, "distillation: the workspace is smaller than "
                                                    "nm_ce_distill_workspace_bytes()");

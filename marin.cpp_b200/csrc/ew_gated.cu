@@ -641,6 +641,13 @@ void require_shape(bool bf16, int64_t T, int D, const std::string& who) {
   NM_REQUIRE(D > 0 && D % 8 == 0, who + ": D must be a positive multiple of 8 (rows are moved in 16-byte pieces)");
   NM_REQUIRE(D <= (bf16 ? 8192 : 4096), who + ": D <= 8192 (bf16 storage) or 4096 (f32)");
 }
+template <class... P>
+void require_element_aligned(bool bf16, const void* gate, const void* dgate, const std::string& who, const P*... f32) {
+  const uintptr_t size = bf16 ? 2 : 4;
+  NM_REQUIRE(reinterpret_cast<uintptr_t>(gate) % size == 0 && reinterpret_cast<uintptr_t>(dgate) % size == 0,
+             who + ": a gate per token must be aligned to its element size");
+  NM_REQUIRE(((reinterpret_cast<uintptr_t>(f32) % 4 == 0) && ...), who + ": statistics and [D] gradients must be 4-byte aligned");
+}
 void require_gate(int gate_kind, const void* gate, const std::string& who) {
   NM_REQUIRE(gate_kind >= kNoGate && gate_kind <= kElementGate, who + ": gate_kind 0 (none), 1 (per token) or 2 (per element)");
   NM_REQUIRE((gate != nullptr) == (gate_kind != kNoGate), who + ": a gate goes with gate_kind 1 or 2, and only with those");
@@ -687,6 +694,7 @@ void gated_tail_fwd(bool bf16, int gate_kind, const void* branch, const void* x_
   NM_REQUIRE(!a_next || g_next, who + ": a_next needs g_next");
   NM_REQUIRE(aligned16(branch, x_in, res_scale, g_post, g_next, x_out, a_next), who + ": every row pointer must be 16-byte aligned");
   NM_REQUIRE(gate_kind != kElementGate || aligned16(gate), who + ": a gate per element must be 16-byte aligned");
+  require_element_aligned(bf16, gate, nullptr, who, rstd_post, rstd_next);
   TailParams p{};
   p.branch = branch, p.x_in = x_in, p.gate = gate, p.res_scale = res_scale, p.g_post = g_post, p.g_next = g_next;
   p.x_out = x_out, p.a_next = a_next, p.rstd_post = rstd_post, p.rstd_next = rstd_next;
@@ -723,6 +731,7 @@ void gated_tail_bwd(bool bf16, int gate_kind, const void* dx_out, const void* da
                who + ": every row pointer must be 16-byte aligned");
     NM_REQUIRE(gate_kind != kElementGate || aligned16(gate, dgate), who + ": a gate per element must be 16-byte aligned");
   }
+  require_element_aligned(bf16, gate, dgate, who, rstd_post, rstd_next, dg_next, dg_post, dres_scale);
   if (sums) {
     NM_REQUIRE(ws != nullptr && reinterpret_cast<uintptr_t>(ws) % 16 == 0, who + ": a 16-byte aligned workspace is required");
     NM_REQUIRE(ws_bytes >= gated_tail_workspace_bytes(T, D), who + ": the workspace is smaller than nm_gated_tail_workspace_bytes()");
