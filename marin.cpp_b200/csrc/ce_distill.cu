@@ -25,17 +25,21 @@ namespace {
 
 using nm::ew::warp_sum;
 using nm::ptx::ex2_approx;
+using nm::ptx::exponent_of;
+using nm::ptx::exponent_step;
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr int kMaxEntries = 512, kMaxExtent = 1 << 30;
 
-// What the rewrite of a row's logits needs: n = a_t 2^(z log2e / tau + e_t) + a_1 2^(z log2e + e_1) - (listed entries)
+// What the rewrite of a row's logits needs: n = a_t 2^(z log2e / tau - r_t) + a_1 2^(z log2e - r_1) - (listed entries), with r
+// the reference exponent round(max z c) that the row's sums count from, and the sums' reciprocals in a. (With the log-sum-exp as
+// the reference its own rounding, half a step of a number of the size of z / tau, would scale every probability.)
 struct alignas(16) DistillRow {
-  float e_t, a_t, e_1, a_1;
+  float r_t, a_t, r_1, a_1;
 };
 __device__ __forceinline__ float dense_part(float z, const DistillRow& f, float tau_log2e) {
-  float n = __fmul_rn(f.a_t, ex2_approx(fmaf(z, tau_log2e, f.e_t)));
-  if (f.a_1 != 0.f) n = fmaf(f.a_1, ex2_approx(fmaf(z, kLog2e, f.e_1)), n);
+  float n = __fmul_rn(f.a_t, ex2_approx(fmaf(z, tau_log2e, -f.r_t)));
+  if (f.a_1 != 0.f) n = fmaf(f.a_1, ex2_approx(fmaf(z, kLog2e, -f.r_1)), n);
   return n;
 }
 
@@ -61,7 +65,7 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
   __shared__ float sm[kStrips][kRowsPerCta], ss[kStrips][kRowsPerCta], s1[kStrips][kRowsPerCta];
   extern __shared__ int32_t entries[];   // per warp: ids [K], masses [K]
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const float inv_tau = __fdiv_rn(1.f, p.tau);
+  const float inv_tau = __fdiv_rn(1.f, p.tau), tau_log2e = __fdiv_rn(kLog2e, p.tau);   // as the logits kernel's
   nm::ptx::release_next();
   nm::ptx::after_previous();
   {
@@ -79,13 +83,13 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
         float nm = m;
 #pragma unroll
         for (int q = 0; q < 8; ++q) nm = fmaxf(nm, tm[q]);
-        const float base = isfinite(nm) ? nm : 0.f, back = isfinite(m) ? m - base : 0.f;   // no sums yet where m is not finite
-        s *= expf(back * inv_tau), o *= expf(back);
+        const float base = isfinite(nm) ? nm : 0.f, from = isfinite(m) ? m : base;   // no sums yet where m is not finite
+        s *= exp2f(exponent_step(from, base, tau_log2e)), o *= exp2f(exponent_step(from, base, kLog2e));
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           if (i + q >= i1) break;
-          s = fmaf(ts[q], expf((tm[q] - base) * inv_tau), s);
-          if (p.tsum1) o = fmaf(to[q], expf(tm[q] - base), o);
+          s = fmaf(ts[q], exp2f(exponent_step(tm[q], base, tau_log2e)), s);
+          if (p.tsum1) o = fmaf(to[q], exp2f(exponent_step(tm[q], base, kLog2e)), o);
         }
         m = nm;
       }
@@ -95,20 +99,22 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
   }
   const int r = blockIdx.x * kRowsPerCta + w;
   if (r >= p.rows) return;
-  float lt, l1;
+  float M, S, S1;    // the maximum and the sums of 2^(z c - exponent_of(M, c)) at the temperature and at 1
   {
-    float m = sm[lane][w], M = m;
+    float m = sm[lane][w];
+    M = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     if (!isfinite(M)) M = 0.f;
-    const float d = isfinite(m) ? m - M : 0.f;   // an empty strip has sums of 0
-    const float S = warp_sum(ss[lane][w] * expf(d * inv_tau));
-    lt = logf(S) + M * inv_tau;
-    l1 = lt;                                     // at temperature 1 one sum serves both
-    if (p.tsum1) l1 = logf(warp_sum(s1[lane][w] * expf(d))) + M;
-    if (lane == 0) p.lse[r] = lt;
+    if (!isfinite(m)) m = M;                     // an empty strip has sums of 0
+    S = warp_sum(ss[lane][w] * exp2f(exponent_step(m, M, tau_log2e)));
+    S1 = S;                                      // at temperature 1 one sum serves both
+    if (p.tsum1) S1 = warp_sum(s1[lane][w] * exp2f(exponent_step(m, M, kLog2e)));
   }
-  const float tau_log2e = kLog2e / p.tau;
+  const float r_t = exponent_of(M, tau_log2e), log2_s = log2f(S);
+  // a log of a sum in nats, counted from M c as it is instead of from its rounding
+  auto log_above_max = [&](float sum, float c) { return fmaf(-kLn2, fmaf(M, c, -exponent_of(M, c)), logf(sum)); };
+  if (lane == 0) p.lse[r] = __fdiv_rn(M, p.tau) + log_above_max(S, tau_log2e);
   int32_t* const id_s = entries + w * 2 * p.K;
   float* const q_s = reinterpret_cast<float*>(id_s + p.K);
   const float wt = p.weight[r];
@@ -116,11 +122,10 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
   const int tg = p.targets ? p.targets[r] : -1;
   const bool labelled = live && p.hard != 0.f && tg >= 0 && tg < p.V && tg != p.ignore_index;
   const int64_t row_k = int64_t(r) * p.K;
-  // the listed entries of this row: id (or -1) and t / tau
-  auto scaled = [&](int k) {
-    const float t = p.logits_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[row_k + k])
-                                  : static_cast<const float*>(p.logits)[row_k + k];
-    return __fdiv_rn(t, p.tau);
+  // the listed entries of this row: id (or -1) and teacher's logit
+  auto teacher = [&](int k) {
+    return p.logits_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[row_k + k])
+                         : static_cast<const float*>(p.logits)[row_k + k];
   };
   __syncwarp();
   float top = -INFINITY;
@@ -128,9 +133,9 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
     const int32_t id = p.ids[row_k + k];
     const bool in = live && id >= 0 && id < p.V;
     id_s[k] = in ? id : -1;
-    if (in && !p.teacher_lse) top = fmaxf(top, scaled(k));
+    if (in && !p.teacher_lse) top = fmaxf(top, teacher(k));
   }
-  float norm = 0.f;
+  float norm = 0.f;   // of the logits counted from `top`, or the given one
   bool any = false;
   if (p.teacher_lse) {
     norm = p.teacher_lse[r];
@@ -140,19 +145,25 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
     any = top != -INFINITY;
     float s = 0.f;
     for (int k = lane; k < p.K; k += 32)
-      if (id_s[k] >= 0 && any) s += expf(scaled(k) - top);
+      if (id_s[k] >= 0 && any) s += expf(__fdiv_rn(teacher(k) - top, p.tau));
     s = warp_sum(s);
-    norm = any ? top + logf(s) : INFINITY;      // nothing listed: every mass is 0
+    norm = any ? logf(s) : INFINITY;            // nothing listed: every mass is 0
   }
+  auto log_mass = [&](int k) {
+    const float t = teacher(k);
+    if (!p.teacher_lse) return (any ? __fdiv_rn(t - top, p.tau) : t) - norm;
+    const float d = __fdiv_rn(t, p.tau);        // and what the quotient lacks, which the difference would show
+    return (d - norm) + (isfinite(d) ? fmaf(-d, p.tau, t) * inv_tau : 0.f);
+  };
   float kl = 0.f, mass = 0.f;
   for (int k = lane; k < p.K; k += 32) {
     const int32_t id = id_s[k];
     float q = 0.f;
     if (id >= 0) {
-      const float lq = scaled(k) - norm;
+      const float lq = log_mass(k);
       q = expf(lq);
       const float z = p.store ? p.store[int64_t(r) * p.ldS + id] : p.zk[row_k + k];
-      if (q != 0.f) kl = fmaf(q, lq - fmaf(z, inv_tau, -lt), kl);
+      if (q != 0.f) kl = fmaf(q, fmaf(-kLn2, fmaf(z, tau_log2e, -r_t) - log2_s, lq), kl);
     }
     q_s[k] = q;
     mass += q;
@@ -164,7 +175,7 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
     float loss = 0.f;
     if (live) {
       loss = p.soft * p.tau * p.tau * kl;
-      if (labelled) loss = fmaf(p.hard, l1 - p.zt[r], loss);
+      if (labelled) loss = fmaf(p.hard, (M - p.zt[r]) + log_above_max(S1, kLog2e), loss);
     }
     p.loss[r] = loss;
     if (p.kl) p.kl[r] = live ? kl : 0.f;
@@ -173,7 +184,7 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
   DistillRow f{0.f, 0.f, 0.f, 0.f};
   const float unit = live ? wt * p.soft * p.tau : 0.f;   // gradient of one unit of teacher mass
   const float hit = labelled ? wt * p.hard : 0.f;
-  if (live) f = DistillRow{-lt * kLog2e, unit * mass, -l1 * kLog2e, hit};
+  if (live) f = DistillRow{r_t, __fdiv_rn(unit * mass, S), exponent_of(M, kLog2e), __fdiv_rn(hit, S1)};
   if (lane == 0) p.rowf[r] = f;
   __syncwarp();
   // the elements of n that are not dense alone, whole: every listed id, and the target where it is not listed

@@ -435,9 +435,9 @@ k_ce_umma(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
           if (row_ok) {
             const int64_t at = int64_t(ni) * p.ldT + grow;
             p.tmax[at] = m;
-            p.tsum[at] = ds.s * ex2_approx(fmaf(ds.m, c, -m * c)) + os * ex2_approx(fmaf(om, c, -m * c));
+            p.tsum[at] = ds.s * ex2_approx(exponent_step(ds.m, m, c)) + os * ex2_approx(exponent_step(om, m, c));
             if (p.tsum1)
-              p.tsum1[at] = ds.s1 * ex2_approx(fmaf(ds.m, kLog2e, -m * kLog2e)) + os1 * ex2_approx(fmaf(om, kLog2e, -m * kLog2e));
+              p.tsum1[at] = ds.s1 * ex2_approx(exponent_step(ds.m, m, kLog2e)) + os1 * ex2_approx(exponent_step(om, m, kLog2e));
           }
         }
       }

@@ -171,8 +171,8 @@ struct WgradArgs {
 void launch_wgrad(const WgradArgs& a, cudaStream_t st);
 
 // ---- the distillation head's contractions (ce_gemm.cu), on the same template
-// z = x W^T: the f32 logits (store [rows, ldS] or nullptr), per 256-column tile max z, sum exp((z - max) / tau) and (tsum1 or
-// nullptr) sum exp(z - max); z[target] -> zt for targets inside [0, V) (targets may be nullptr).
+// z = x W^T: the f32 logits (store [rows, ldS] or nullptr), per 256-column tile m = max z, the sum of 2^(z c - round(m c)) with
+// c = log2e / tau and (tsum1 or nullptr) the same with c = log2e; z[target] -> zt for targets inside [0, V) (targets may be nullptr).
 struct DistillLogitsArgs {
   const void* x; const void* w; const int32_t* targets;
   int rows, D, V;

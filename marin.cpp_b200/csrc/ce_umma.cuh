@@ -138,8 +138,11 @@ __device__ __forceinline__ void epi_logits_chunk(const GemmParams& p, float* v, 
   }
 }
 
-// The distillation head's statistics: the maximum of the raw logits, sum exp((z - max) / tau) and, when wanted, sum
-// exp(z - max), online as above. The f32 logits leave through the staging tile (the caller).
+// The distillation head's statistics: the maximum m of the raw logits and, with c = log2e / tau and R(m) = round(m c) (exponent_of), the
+// sum of 2^(z c - R(m)); when wanted the same at c = log2e. R is a number that every later step recomputes from m and measures
+// from, not an approximation of m c: a sum moves to another maximum by 2^(R(old) - R(new)), which is exactly 1 when the
+// maximum stands (with 2^(old c - R(new)) a sum picks the rounding of R up at every chunk: 2e-4 of it at z = 50, tau = 0.05).
+// The f32 logits leave through the staging tile (the caller).
 struct DistillRowState {
   float m, s, s1, zt;
   bool hit;
@@ -154,11 +157,11 @@ __device__ __forceinline__ void epi_distill_chunk(const GemmParams& p, const flo
 #pragma unroll
     for (int j = 4; j < 32; ++j) t[j & 3] = fmaxf(t[j & 3], v[j]);
     m = fmaxf(st.m, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-    const float neg = -m * c;
+    const float neg = -exponent_of(m, c);
 #pragma unroll
     for (int j = 0; j < 32; ++j) a[j & 3] += ex2_approx(fmaf(v[j], c, neg));
     if (p.tsum1) {                          // uniform over the launch
-      const float neg1 = -m * kLog2e;
+      const float neg1 = -exponent_of(m, kLog2e);
 #pragma unroll
       for (int j = 0; j < 32; ++j) b[j & 3] += ex2_approx(fmaf(v[j], kLog2e, neg1));
     }
@@ -171,14 +174,14 @@ __device__ __forceinline__ void epi_distill_chunk(const GemmParams& p, const flo
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       if (j < ncols) {
-        a[j & 3] += ex2_approx(fmaf(v[j], c, -m * c));
-        if (p.tsum1) b[j & 3] += ex2_approx(fmaf(v[j], kLog2e, -m * kLog2e));
+        a[j & 3] += ex2_approx(fmaf(v[j], c, -exponent_of(m, c)));
+        if (p.tsum1) b[j & 3] += ex2_approx(fmaf(v[j], kLog2e, -exponent_of(m, kLog2e)));
       }
     }
   }
   // st.m == -inf on the first chunk: ex2(-inf) = 0 and the sums are 0
-  st.s = st.s * ex2_approx(fmaf(st.m, c, -m * c)) + ((a[0] + a[1]) + (a[2] + a[3]));
-  if (p.tsum1) st.s1 = st.s1 * ex2_approx(fmaf(st.m, kLog2e, -m * kLog2e)) + ((b[0] + b[1]) + (b[2] + b[3]));
+  st.s = st.s * ex2_approx(exponent_step(st.m, m, c)) + ((a[0] + a[1]) + (a[2] + a[3]));
+  if (p.tsum1) st.s1 = st.s1 * ex2_approx(exponent_step(st.m, m, kLog2e)) + ((b[0] + b[1]) + (b[2] + b[3]));
   st.m = m;
   if (tg >= col0 && tg < col0 + 32) {
     const int jt = tg - col0;

@@ -408,4 +408,11 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return r;
 }
 
+// The reference that sums of 2^(z c - .) with maximum m count from, and the exponent that takes such a sum from one maximum to
+// another: 0 when they are equal, whatever m c was rounded to.
+__device__ __forceinline__ float exponent_of(float m, float c) { return __fmul_rn(m, c); }
+__device__ __forceinline__ float exponent_step(float from, float to, float c) {
+  return __fsub_rn(exponent_of(from, c), exponent_of(to, c));
+}
+
 }  // namespace nm::ptx
