@@ -123,11 +123,6 @@ __device__ __forceinline__ float scalar_of(const void* p, int64_t i, bool bf16) 
   return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 
-// sigmoid(g) and 1 - sigmoid(g) of two gates. The exponent stops at 126: beyond it the open part is 2^-126 instead of 0,
-// and e * on stays a number (a NaN passes through).
-struct Gate2 {
-  Two on, off;
-};
 __device__ __forceinline__ float gate_exponent(float a) {
   float r;
   asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(r) : "f"(a));
@@ -139,14 +134,6 @@ __device__ __forceinline__ float rcp_approx(float a) {
   return r;
 }
 constexpr float kLog2e = 1.4426950408889634f, kLargest = 3.402823466e38f;
-__device__ __forceinline__ Gate2 gate_of(Two g) {
-  const Two e = two(nm::ptx::ex2_approx(gate_exponent(__fmul_rn(g.x, -kLog2e))),
-                    nm::ptx::ex2_approx(gate_exponent(__fmul_rn(g.y, -kLog2e))));
-  Gate2 r;
-  r.on = two(rcp_approx(__fadd_rn(1.f, e.x)), rcp_approx(__fadd_rn(1.f, e.y)));
-  r.off = mul(e, r.on);
-  return r;
-}
 
 // What x_out is made of, s x + y / (1 + exp(-gate)), takes expf and a quotient rounded once: x_out is rounded to the storage
 // type, and in bf16 a value next to a tie lands a whole step (2^-8) away for a difference of 2^-24, which every sum over x_out
@@ -178,6 +165,29 @@ __device__ __forceinline__ Two through(Two y, const Opening& o) {   // y / (1 + 
   return fma2(rest, o.r, q);
 }
 __device__ __forceinline__ float both(Two v) { return v.x + v.y; }
+
+// sigmoid(g) and 1 - sigmoid(g) of two gates, for the gradients. f32 storage shows all bits of them and takes what x_out takes:
+// within 6 and 7 half steps. In bf16 storage they are factors of results that are rounded to 2^-8: ex2.approx of a rounded product
+// (|g| half steps of f32) and rcp.approx. There the exponent stops at 126: beyond it the open part is 2^-126 instead of 0, and
+// e * on stays a number (a NaN passes through).
+struct Gate2 {
+  Two on, off;
+};
+template <bool BF16>
+__device__ __forceinline__ Gate2 gate_of(Two g) {
+  Two e;
+  Gate2 r;
+  if constexpr (BF16) {
+    e = two(nm::ptx::ex2_approx(gate_exponent(__fmul_rn(g.x, -kLog2e))),
+            nm::ptx::ex2_approx(gate_exponent(__fmul_rn(g.y, -kLog2e))));
+    r.on = two(rcp_approx(__fadd_rn(1.f, e.x)), rcp_approx(__fadd_rn(1.f, e.y)));
+  } else {
+    e = two(exp_of_minus(g.x), exp_of_minus(g.y));
+    r.on = through<false>(two(1.f, 1.f), opening_of(g));
+  }
+  r.off = mul(e, r.on);
+  return r;
+}
 
 struct TailParams {
   const void* branch; const void* x_in; const void* gate; const void* res_scale; const void* g_post; const void* g_next;
@@ -459,7 +469,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
     Gate2 tgate{two(1.f, 1.f), two(0.f, 0.f)};
     Opening token;
     if constexpr (GATE == kTokenGate) {
-      tgate = gate_of(two(mine.gate, mine.gate));
+      tgate = gate_of<BF16>(two(mine.gate, mine.gate));
       token = opening_of(two(mine.gate, mine.gate));
     }
     mine = scalars_of(r0 + rg.groups);
@@ -554,7 +564,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
         if constexpr (GATE == kTokenGate) t = mul2(t, tgate.on);
         Two off;
         if constexpr (GATE == kElementGate) {
-          const Gate2 z = gate_of(g.pair(q));
+          const Gate2 z = gate_of<BF16>(g.pair(q));
           t = mul2(t, z.on);
           off = z.off;
         }
