@@ -138,11 +138,11 @@ __device__ __forceinline__ void epi_logits_chunk(const GemmParams& p, float* v, 
   }
 }
 
-// The distillation head's statistics: the maximum m of the raw logits and, with c = log2e / tau and R(m) = round(m c) (exponent_of), the
-// sum of 2^(z c - R(m)); when wanted the same at c = log2e. R is a number that every later step recomputes from m and measures
-// from, not an approximation of m c: a sum moves to another maximum by 2^(R(old) - R(new)), which is exactly 1 when the
-// maximum stands (with 2^(old c - R(new)) a sum picks the rounding of R up at every chunk: 2e-4 of it at z = 50, tau = 0.05).
-// The f32 logits leave through the staging tile (the caller).
+// The distillation head's statistics: the maximum m of the raw logits and, with c = log2e / tau and R(m) = round(m c)
+// (exponent_of), the sum of 2^(z c - R(m)); when wanted the same at c = log2e. R is a number that every later step recomputes
+// from m and measures from, not an approximation of m c: a sum moves to another maximum by 2^(R(old) - R(new)), which is exactly
+// 1 when the maximum stands (with 2^(old c - R(new)) a sum picks the rounding of R up at every chunk: 2e-4 of it at z = 50,
+// tau = 0.05). The f32 logits leave through the staging tile (the caller).
 struct DistillRowState {
   float m, s, s1, zt;
   bool hit;

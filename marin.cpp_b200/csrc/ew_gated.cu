@@ -32,7 +32,7 @@ namespace {
 // the same bits. Written as one asm block each: with the values held as 64-bit registers between the operations (ew_rows.cuh)
 // the moves that put single results side by side ate the gain. Backward, 65536 x 2048: 279 million warp instructions with
 // plain arithmetic, 243 million packed (390 -> 387 us under the power cap, 349 us at full clock either way: HBM; before the
-// quotient below was rounded once). Forward, the same size: 232 -> 231 us, 251 -> 250 us under the cap.
+// quotient below was corrected). Forward, the same size: 232 -> 231 us, 251 -> 250 us under the cap.
 struct Two {
   float x, y;
 };
@@ -135,11 +135,14 @@ __device__ __forceinline__ float rcp_approx(float a) {
 }
 constexpr float kLog2e = 1.4426950408889634f, kLargest = 3.402823466e38f;
 
-// What x_out is made of, s x + y / (1 + exp(-gate)), takes expf and a quotient rounded once: x_out is rounded to the storage
+// What x_out is made of, s x + y / (1 + exp(-gate)), takes expf and a quotient of half a step: x_out is rounded to the storage
 // type, and in bf16 a value next to a tie lands a whole step (2^-8) away for a difference of 2^-24, which every sum over x_out
 // shows. With ex2.approx of a rounded product and rcp.approx the f32 sums stood up to 2e-5 from those of the formula's own f32
-// operations, now 3e-7 (12 % of the forward and 6 % of the backward under the power cap). The quotient is q = y r, r about the
-// reciprocal of 1 + exp(-gate), refined by its remainder. The gate stops at -87, where the quotient is as good as 0; a NaN
+// operations, now 3e-7 (12 % of the forward and 6 % of the backward under the power cap). The quotient y / b is P. Markstein's
+// for machines with a fused multiply-add (Computation of elementary functions on the IBM RISC System/6000 processor, IBM J. Res.
+// Develop. 34, 1990): q = y r with r about 1 / b, then q + (y - q b) r, whose remainder is rounded once. With r and q each within
+// 2^-22 (rcp.approx 1 ulp, the product) what the one correction leaves is under 2^-43 before the last rounding: half a step and
+// a little, not always the nearest value. The gate stops at -87, where the quotient is as good as 0; a NaN
 // passes through. The remainder of an infinite y is inf - inf; INF makes it a number and the quotient infinite. The backward
 // does without: the row's rstd_next is 0 and 0 inf = NaN reaches all its gradients either way. A part that the call leaves out
 // is a factor of one (exact), so nothing branches on it. Both directions get the same bits from these.
@@ -405,7 +408,7 @@ __device__ __forceinline__ void write_quad_partial(const Two (&dg)[N][2], const 
 // 65536 x 2048 bf16 with a gate per element (floor 328 us at the copy rate): 811 us with the gate's two parts kept and eight
 // columns at a time (spills), 414 us as quads without spills, 353 us with plain arithmetic instead of
 // packed 64-bit registers and the next batch fetched before a batch is worked on (6.1 TB/s); 364-370 us, 414-426 us under the
-// power cap, since the gate's quotient is rounded once. Sixteen columns per thread beat eight (439 us).
+// power cap, since the gate's quotient is corrected. Sixteen columns per thread beat eight (439 us).
 template <bool BF16, int PP, int GATE>
 __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gated_bwd(const TailParams p) {
   using namespace nm::ptx;
