@@ -536,7 +536,8 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
     }
     float sums[3] = {both(sxa), both(suh), both(sux)};
     group_sum<3>(sums, rg, red, flip);
-    const float cn = -(r_n * r_n) * r_n * (sums[0] * inv_d);
+    // the sum grows with x_out as r_n shrinks: r_n^3 by itself is 0 in f32 from x_out = 10^15 on
+    const float cn = -(sums[0] * inv_d * r_n * r_n * r_n);
     const float sum_um = fmaf(cn, sums[2], sums[1]);    // without the gate when it is the token's
     const float token_on = tgate.on.x, token_off = tgate.off.x;
     if constexpr (GATE == kTokenGate) {
@@ -546,8 +547,8 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
         else static_cast<float*>(p.dgate)[tr.row0 + r0] = d;
       }
     }
-    // -r_p^3 sum(branch p) / D with sum(branch p) = sum(u m) / r_p
-    const float cp = post ? -(r_p * r_p) * ((GATE == kTokenGate ? sum_um * token_on : sum_um) * inv_d) : 0.f;
+    // -r_p^2 sum(branch p) / D with sum(branch p) = sum(u m) / r_p; the third r_p goes to the branch, whose size it has
+    const float cp = post ? -((GATE == kTokenGate ? sum_um * token_on : sum_um) * inv_d * r_p) : 0.f;
     const Two c_n = two(cn, cn), c_p = two(cp, cp);
     const int64_t out0 = ((tr.row0 + r0) * quads + first) * int64_t(Q::kBytes);
 #pragma unroll
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gate
         dgp[j][q] = fma2(t, b.pair(q), dgp[j][q]);
         const Two pr = mul2(gp.pair(q), t);
         if constexpr (GATE == kElementGate) vg[q] = mul2(mul2(pr, b.pair(q)), off);
-        vb[q] = fma2(c_p, b.pair(q), pr);
+        vb[q] = fma2(c_p, mul2(b.pair(q), rp), pr);
       }
       constexpr int kStep = 32 * int(Q::kBytes);
       Q o;
