@@ -369,7 +369,16 @@ constexpr int kNoKey = INT_MAX;
 // Measured for the whole call: 131072 tokens of width 2048 (ids falling as 1 / rank), windows of 64 rows 297 us, of 32 rows
 // 305 us (twice the cut pieces); 2125 tokens of width 768 in f32, windows of 32 rows 26 us, of 16 rows 20.5 us (a short
 // section waits for the longest window).
-inline int window_for(int64_t n) { return n > 32768 ? 64 : n > 2560 ? 32 : 16; }
+constexpr int64_t kMost16 = 2560, kMost32 = 32768;   // tokens in windows of 16 and of 32 rows
+inline int window_for(int64_t n) { return n > kMost32 ? 64 : n > kMost16 ? 32 : 16; }
+inline int64_t windows_of(int64_t n) { return (n + window_for(n) - 1) / window_for(n); }
+// The most windows of any section of up to n tokens: a workspace planned for the longest call serves every shorter one.
+inline int64_t windows_up_to(int64_t n) {
+  int64_t most = windows_of(n);
+  if (n > kMost16) most = std::max(most, windows_of(kMost16));
+  if (n > kMost32) most = std::max(most, windows_of(kMost32));
+  return most;
+}
 
 struct ReduceParams {
   const void* dy;
@@ -650,7 +659,7 @@ struct BwdRegions {
   uint64_t bytes;
 };
 BwdRegions bwd_layout(int64_t T, int D, void* base) {
-  const int64_t n = std::min(T, kSection), windows = (n + window_for(n) - 1) / window_for(n);
+  const int64_t n = std::min(T, kSection), windows = windows_up_to(n);
   ce::Arena arena(base);
   BwdRegions r{};
   r.keys = arena.take<int32_t>(uint64_t(n));
@@ -777,7 +786,7 @@ void embed_bwd(bool bf16, const void* dy, const int32_t* tokens, float* dtable, 
     rp.dy = static_cast<const uint8_t*>(dy) + t0 * D * (bf16 ? 2 : 4);
     rp.keys = r.keys, rp.pos = r.pos, rp.chains = r.chains, rp.part = r.part, rp.dtable = dtable, rp.scale = scale;
     rp.n = n, rp.V = V, rp.D = D, rp.G = threads_per_row(D / 8), rp.accumulate = add;
-    rp.win = window_for(n), rp.windows = (n + rp.win - 1) / rp.win;
+    rp.win = window_for(n), rp.windows = int(windows_of(n));
     rp.wide = wide;
     const int groups = kThreads / rp.G;
     const dim3 rg(unsigned((rp.windows + groups - 1) / groups), unsigned((D / 8 + rp.G - 1) / rp.G));
