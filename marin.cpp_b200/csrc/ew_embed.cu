@@ -366,17 +366,24 @@ __global__ void __launch_bounds__(kSortThreads, 1) k_embed_sort(const SortParams
 // runs are never cut, no window has more than 2.5 win rows to read, and a cut costs 8 bytes of f32 traffic per column
 // for at least win / 2 rows read.
 constexpr int kNoKey = INT_MAX;
-// Measured for the whole call: 131072 tokens of width 2048 (ids falling as 1 / rank), windows of 64 rows 297 us, of 32 rows
-// 305 us (twice the cut pieces); 2125 tokens of width 768 in f32, windows of 32 rows 26 us, of 16 rows 20.5 us (a short
-// section waits for the longest window).
-constexpr int64_t kMost16 = 2560, kMost32 = 32768;   // tokens in windows of 16 and of 32 rows
-inline int window_for(int64_t n) { return n > kMost32 ? 64 : n > kMost16 ? 32 : 16; }
-inline int64_t windows_of(int64_t n) { return (n + window_for(n) - 1) / window_for(n); }
+// Rows per window: many windows keep every SM busy and no CTA waits long, few of them cut fewer runs (8 bytes per column and
+// cut). Whole calls of 16 / 32 / 64 rows in us, ids falling as 1 / rank, replayed from a graph:
+//   2000 x 512 bf16, added 17 / 21 / 30     8000 x 64 bf16, added 23 / 26 / 34       16384 x 256 bf16 43 / 50 / 56
+//   4000 x 512 bf16, added 26 / 32 / 33     16000 x 64 bf16, added 26 / 28 / 36      16000 x 768 f32, added 50 / 44 / 47
+//   32768 x 2048 bf16 218 / 217 / 222       48000 x 512 bf16, added 52 / 49 / 58     65536 x 2048 bf16 257 / 244 / 246
+//   64000 x 768 f32, added 116 / 120 / 142  98304 x 1024 f32 234 / 230 / 237         98304 x 2048 bf16 294 / 273 / 271
+//   131072 x 512 bf16 120 / 112 / 116       131072 x 1024 f32 276 / 268 / 281        131072 x 2048 bf16 330 / 301 / 293
+// and of a single id, which is cut at every edge: 16384 x 512 36 / 29 / 28, 131072 x 2048 383 / 239 / 175. So 16 rows for short
+// sections, as long as the cut pieces' rows (8 D n / 16 bytes of workspace) stay under 2.5 MiB, and 64 for a nearly full one.
+constexpr int64_t kMost16 = 16384, kMost16Elements = int64_t(5) << 20, kMost32 = 98304;
+inline int64_t most16(int D) { return std::min(kMost16, kMost16Elements / D); }   // tokens in windows of 16 rows
+inline int window_for(int64_t n, int D) { return n > kMost32 ? 64 : n > most16(D) ? 32 : 16; }
+inline int64_t windows_of(int64_t n, int D) { return (n + window_for(n, D) - 1) / window_for(n, D); }
 // The most windows of any section of up to n tokens: a workspace planned for the longest call serves every shorter one.
-inline int64_t windows_up_to(int64_t n) {
-  int64_t most = windows_of(n);
-  if (n > kMost16) most = std::max(most, windows_of(kMost16));
-  if (n > kMost32) most = std::max(most, windows_of(kMost32));
+inline int64_t windows_up_to(int64_t n, int D) {
+  int64_t most = windows_of(n, D);
+  if (n > most16(D)) most = std::max(most, windows_of(most16(D), D));
+  if (n > kMost32) most = std::max(most, windows_of(kMost32, D));
   return most;
 }
 
@@ -659,7 +666,7 @@ struct BwdRegions {
   uint64_t bytes;
 };
 BwdRegions bwd_layout(int64_t T, int D, void* base) {
-  const int64_t n = std::min(T, kSection), windows = windows_up_to(n);
+  const int64_t n = std::min(T, kSection), windows = windows_up_to(n, D);
   ce::Arena arena(base);
   BwdRegions r{};
   r.keys = arena.take<int32_t>(uint64_t(n));
@@ -786,7 +793,7 @@ void embed_bwd(bool bf16, const void* dy, const int32_t* tokens, float* dtable, 
     rp.dy = static_cast<const uint8_t*>(dy) + t0 * D * (bf16 ? 2 : 4);
     rp.keys = r.keys, rp.pos = r.pos, rp.chains = r.chains, rp.part = r.part, rp.dtable = dtable, rp.scale = scale;
     rp.n = n, rp.V = V, rp.D = D, rp.G = threads_per_row(D / 8), rp.accumulate = add;
-    rp.win = window_for(n), rp.windows = int(windows_of(n));
+    rp.win = window_for(n, D), rp.windows = int(windows_of(n, D));
     rp.wide = wide;
     const int groups = kThreads / rp.G;
     const dim3 rg(unsigned((rp.windows + groups - 1) / groups), unsigned((D / 8 + rp.G - 1) / rp.G));
