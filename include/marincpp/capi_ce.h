@@ -148,12 +148,17 @@ int nm_ce_sampled_head(int rounding, int logits_store, const void* x, const void
  *      against a teacher's listed logits [T, K] (ids outside [0, V) are padding), q their softmax at temperature tau, or with
  *      teacher_lse [T] (log sum exp(. / tau) over the teacher's whole vocabulary) their true masses; and its gradients
  *      dx [T, D] bf16 (accumulate_dx: added to) and dw [V, D] f32 (added to). x, w bf16, D % 8 == 0; teacher_dtype 0 f32,
- *      1 bf16; K 1 .. 512; V and the rows of a chunk at most 2^30. NULL: teacher_lse, targets (when hard_weight is 0), kl_tok, lse (log sum exp(z / tau)),
- *      loss_partial, dx, dw, and grad_scale when both are NULL. dx may be x when it does not accumulate. forward_only != 0:
- *      no gradients, and a workspace without a logits store. Same bits for the same call and chunk_rows. workspace: 256-byte
- *      aligned, nm_ce_distill_workspace_bytes (0 on error) with the same arguments; word 0 is the wait status
- *      (nm_ce_device_status). Nothing is allocated; the call can be captured into a CUDA graph (make the first call on a
- *      device outside a capture). --------------------------------------------------------------------------------- */
+ *      1 bf16; K 1 .. 512; V and the rows of a chunk at most 2^30. NULL: teacher_lse, targets (when hard_weight is 0),
+ *      kl_tok, lse (log sum exp(z / tau)), loss_partial, dx, dw, and grad_scale when both are NULL. dx may be x when it does
+ *      not accumulate. forward_only != 0: no gradients, and a workspace without a logits store.
+ *      Precision: losses and statistics are f32 throughout. dw: the gradient n of the logits as two bf16 terms (2^-17), added up
+ *      over at most 1152 rows in the tensor core's accumulator, which truncates: 2e-6 to 4e-6 from float64 (2-norm). dx: chunks of
+ *      more than 128 rows take n rounded to bf16 once (2.3e-3 from float64, of which the storage of dx itself is 1.7e-3; up
+ *      to 1.3e-4 small where one accumulator runs over a vocabulary of 128256), shorter ones both terms (1.7e-3); so a row's dx
+ *      may differ in its last bit between calls of 128 and of 129 rows.
+ *      Same bits for the same call and chunk_rows. workspace: 256-byte aligned, nm_ce_distill_workspace_bytes (0 on error) with
+ *      the same arguments, one for each of the calls that may overlap; word 0 is the wait status (nm_ce_device_status). Nothing
+ *      is allocated; the call can be captured into a CUDA graph (make the first call on a device outside a capture). ------ */
 uint64_t nm_ce_distill_workspace_bytes(int64_t T, int D, int V, int K, int chunk_rows, int forward_only);
 int nm_ce_distill(int teacher_dtype, const void* x, const void* w, const int32_t* teacher_ids, const void* teacher_logits,
                   const float* teacher_lse, const int32_t* targets, const float* weight, const float* grad_scale,

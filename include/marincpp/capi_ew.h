@@ -39,14 +39,17 @@ int nm_norm_bwd_test_timeout(int64_t limit_cycles, void* stream);
 /* ---- embedding (the reference's trunk has its own, src/kernels/elementwise/embed.cu; names and workspace here are this
  * library's). dtype: storage of table / out / dy, 1 = bf16, 0 = f32. D % 8 == 0, D <= 65536, rows contiguous and
  * 16-byte aligned.
- * forward:  out[t, :] = round(scale * table[tokens[t], :]), one rounding; a token outside [0, V) gives a row of zeros. */
+ * forward:  out[t, :] = round(scale * table[tokens[t], :]), the f32 product rounded to the storage; a token outside [0, V)
+ * gives a row of zeros. */
 int nm_embed_fwd(int dtype, const void* table, const int32_t* tokens, void* out, float scale, int64_t T, int D, int V,
                  void* stream);
 /* backward: dtable[v, :] (f32 [V, D]) = or += scale * sum over t with tokens[t] = v of dy[t, :]. accumulate 0 writes all
  * V rows (zeros for absent tokens), 1 adds and leaves absent rows untouched (a tied head's dW may be the buffer); tokens
  * outside [0, V) contribute nothing. Sums are f32 in an order that depends on the tokens alone: the same call gives the
- * same bits. workspace: nm_embed_bwd_workspace_bytes (0 on error), 256-byte aligned, scratch between calls; calls that may
- * overlap need one each. Nothing is allocated; the calls can be captured into a CUDA graph. */
+ * same bits. With accumulate a row's sum is added at L2, where values below 2^-126 count as 0. workspace:
+ * nm_embed_bwd_workspace_bytes (0 on error; does not fall as T grows, so that of the longest call serves all), 256-byte
+ * aligned, scratch between calls; calls that may overlap need one each. Nothing is allocated; the calls can be captured
+ * into a CUDA graph. */
 uint64_t nm_embed_bwd_workspace_bytes(int64_t T, int D, int V);
 int nm_embed_bwd(int dtype, const void* dy, const int32_t* tokens, float* dtable, float scale, int accumulate, int64_t T,
                  int D, int V, void* workspace, uint64_t workspace_bytes, void* stream);
@@ -58,7 +61,8 @@ int nm_embed_bwd(int dtype, const void* dy, const int32_t* tokens, float* dtable
  *   y = g_post ? g_post * branch * rstd_post : branch        rstd_post = 1 / sqrt(mean(branch^2) + eps)
  *   x_out = round(res_scale * x_in + sigmoid(gate) * y)      gate_kind 0: no gate (NULL), 1: gate [T], 2: gate [T, D]
  *   a_next = round(g_next * x_out * rstd_next)               rstd_next = 1 / sqrt(mean(x_out^2) + eps), of the rounded x_out
- * NULL: res_scale ([D]; 1), g_post ([D]; no post-norm), a_next (then g_next too), rstd_post / rstd_next (not returned).
+ * NULL: res_scale ([D]; 1), g_post ([D]; no post-norm, and rstd_post is left as it was), a_next (then g_next too),
+ * rstd_post / rstd_next (not returned). Statistics and [D] gradients are 4-byte aligned.
  * x_out may be x_in and a_next may be branch. */
 int nm_gated_tail_fwd(int dtype, int gate_kind, const void* branch, const void* x_in, const void* gate,
                       const void* res_scale, const void* g_post, const void* g_next, void* x_out, void* a_next,

@@ -211,8 +211,10 @@ __global__ void __launch_bounds__(32 * kRowsPerCta) k_distill_rows(const Distill
 }
 
 // Student logits of the listed ids for a call that stores none: one f32 dot product of x_t and W[id] each. A warp takes four
-// entries of a row at a time, a lane every 32nd 16-byte piece of the two rows. 2125 x 16 entries of width 512: 11 us of
-// latency, where storing and gathering the logits would move a gigabyte.
+// entries of a row at a time, a lane every 32nd 16-byte piece of the two rows. The only form there is for such a call, whatever
+// K: storing the logits would need the large workspace that the caller did not give, and 4 T V bytes of traffic each way against
+// 2 T K D here. The whole call in us for K = 1 / 16 / 64 / 128 / 256 / 512: 2125 x 512 x 128256 222 / 225 / 246 / 271 / 318 / 410;
+// 8192 x 2048 x 128256 3061 / 3073 / 3412 / 3855 / 4697 / 6335; 1000 x 1024 x 32000 85 / 85 / 100 / 118 / 163 / 242.
 constexpr int kDotEntries = 4;
 __global__ void __launch_bounds__(256) k_distill_dots(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ w,
                                                       const int32_t* __restrict__ ids, const float* __restrict__ weight,

@@ -620,8 +620,11 @@ void launch_distill_logits(const DistillLogitsArgs& a, cudaStream_t st) {
 
 // Shares of the dX contraction: one CTA per tile leaves SMs idle when a call has few tiles, or a last wave with few of them.
 // The number with the fewest K blocks per SM is taken, a share counting 24 blocks more for its epilogue and the reading of its
-// sums (16 rows x 512, 8256 ids, the whole call: 1 share 128 us, 4 63 us, 8 and 16 46 to 55 us, 43 58 us); the sums take at
-// most kMaxDxShareRows x D f32.
+// sums. Logits, gradient pass and dX in us, the rule's choice of shares first: 16 x 512 x 8256 16: 32 (1: 94, 4: 43, 8: 35);
+// 128 x 1024 x 64256 16: 114 (1: 765, 8: 153); 600 x 768 x 32000 9: 118 (1: 249, 8: 119, 10: 136); 1024 x 2048 x 128256 9: 1179
+// (1: 1567, 2: 1175, 5: 1293); 2125 x 512 x 128256 4: 1003 (1: 1566, 2: 1184, 8: 1012); 4096 x 512 x 50000 2: 739 (1: 883, 3:
+// 803, 4: 763); 8192 x 2048 x 128256 2: 8427 (1: 8688, 4: 8570); of 1 to 16 shares at ten shapes it is the fastest or within
+// 0.4 % of it. The sums take at most kMaxDxShareRows x D f32.
 int distill_dgrad_shares(int rows, int D, int V) {
   const int64_t tiles = int64_t((rows + BM - 1) / BM) * ((D + BN - 1) / BN), sms = sm_count();
   const int64_t kb = (V + BK - 1) / BK * (rows <= kTwoTermDxRows ? 2 : 1);

@@ -79,8 +79,8 @@ using nm::ptx::release_next;
 // ------------------------------------------------------------------------------------------------ forward
 // G threads side by side on a row (eight elements each); a row group takes `batches` times kFwdRows consecutive rows, the
 // loads of a batch in flight while the one before it is stored. Bound by HBM: the output is written once, past the L2 (the
-// frequent rows of the table are read from there again and again). 131072 x 2048 bf16, ids falling as 1 / rank (35 thousand
-// distinct rows): 117 us, 5.8 TB/s; batches of three rows 118 us, of four 122 us, one batch of four rows per group 128 us.
+// frequent rows of the table are read from there again and again). 131072 x 2048 bf16, ids falling as 1 / rank (32 thousand
+// distinct rows): 117 us, 5.7 TB/s; batches of three rows 118 us, of four 122 us, one batch of four rows per group 128 us.
 constexpr int kFwdRows = 2, kFwdMaxBatches = 8;
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads, BF16 ? 6 : 4) k_embed_fwd(const void* __restrict__ table, const int32_t* __restrict__ tokens,
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) k_embed_rank(const SortParams p) {
 // vocabulary is larger than the section). It needs the tokens, not their order, so it runs beside the sort: it does not wait
 // for the launch before it until it has done its work. The vocabulary is dealt to the CTAs (a power of two of them) in
 // blocks of eight rows, because frequent ids lie together; a CTA marks the tokens of its share (10 us for 131072 tokens), then
-// writes. Bound by HBM: 850 MB in 137 us; dealt in contiguous ranges 148 us.
+// writes. Bound by HBM: 786 MB in 137 us; dealt in contiguous ranges 148 us.
 constexpr int kZeroThreads = 1024, kZeroSlab = 65536;   // rows whose presence a CTA marks at a time (8 KiB of bits)
 struct ZeroParams {
   const int32_t* tokens;
@@ -421,7 +421,7 @@ __device__ __forceinline__ int first_owned(const Key& key, int b, int win, int V
 
 // A thread's pieces of the rows to come travel through its own slots of a ring in shared memory (cp.async, no barrier:
 // nobody else reads them), 64 KiB in flight per CTA: what a window waits for is a few round trips, and registers do not
-// limit how many rows are on their way. Bound by HBM: 131072 x 2048 bf16 into 35 thousand rows 128 us (740 MB, 5.8 TB/s);
+// limit how many rows are on their way. Bound by HBM: 131072 x 2048 bf16 into 32 thousand rows 128 us (795 MB, 6.2 TB/s);
 // with loads into registers 175 us.
 template <bool BF16>
 struct Ring {

@@ -12,7 +12,7 @@
 // sigmoid(g) = r = 1 / (1 + e) and 1 - sigmoid(g) = e r with e = exp(-g): no cancellation at either end.
 // Row groups and batch ring as in ew_rows.cuh, a CTA per part of consecutive rows. What bounds them is HBM (10 and 16 bytes
 // per element in bf16 with a gate per element), and under the board's power cap, at 1.7 GHz, the issue slots. Forward,
-// 65536 x 2048: 231 us (5.8 TB/s), 250 us under the cap; the backward's figures stand at its kernel.
+// 65536 x 2048: 229 us (5.9 TB/s), 244 to 260 us under the cap; the backward's figures stand at its kernel.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -407,7 +407,7 @@ __device__ __forceinline__ void write_quad_partial(const Two (&dg)[N][2], const 
 // nearly all of the SM's memory a spilled register is read back from L2, so the registers decide the form. Measured for
 // 65536 x 2048 bf16 with a gate per element (floor 328 us at the copy rate): 811 us with the gate's two parts kept and eight
 // columns at a time (spills), 414 us as quads without spills, 353 us with plain arithmetic instead of
-// packed 64-bit registers and the next batch fetched before a batch is worked on (6.1 TB/s); 364-370 us, 414-426 us under the
+// packed 64-bit registers and the next batch fetched before a batch is worked on (6.1 TB/s); 359-370 us, 402-426 us under the
 // power cap, since the gate's quotient is corrected. Sixteen columns per thread beat eight (439 us).
 template <bool BF16, int PP, int GATE>
 __global__ void __launch_bounds__(kGroupThreads, PP <= 2 && BF16 ? 2 : 1) k_gated_bwd(const TailParams p) {
